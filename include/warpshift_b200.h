@@ -259,6 +259,119 @@ WS_API int ws_tensor_hashes(const void* const* ptrs, const uint64_t* nbytes, uin
  * completes. */
 WS_API int ws_selftest_wait_timeout(uint32_t polls, int device, void* stream, uint32_t* device_errors);
 
+/* ---------------------------------------------------------------------------
+ * Operators on rows of logits: what a resident teacher answers with, and what a
+ * student learns from it. No counterpart in the reference, whose server hands
+ * logits to SGLang; its acceptance check compares greedy tokens and
+ * log-probabilities on the host (scripts/validate.py:142-155).
+ *
+ * All of them enqueue on `stream` of `device` and return without waiting: they
+ * allocate nothing, keep nothing between calls, need no workspace, and can be
+ * captured into a CUDA graph. Device memory that a call names stays the caller's
+ * and has to live until the call's work is done. Zero rows are a call that does nothing. */
+#define WS_DTYPE_BF16 0
+#define WS_DTYPE_FP16 1
+#define WS_DTYPE_FP32 2
+#define WS_MAX_VOCAB (1u << 20)      /* longest row */
+#define WS_MAX_LOGIT_ROWS (1u << 27) /* most rows of a call */
+#define WS_TOP_MAX_K 256             /* longest teacher record of a row */
+
+/* `rows` rows of `vocab` contiguous elements each. Row r starts at element
+ * (r / inner) * stride_outer + (r % inner) * stride_inner of `data`, so that the
+ * rows of a 3-D slice (logits[:, :-1]) need no copy. Rows that are read may
+ * overlap; rows that are written must not. Any alignment of the element type will
+ * do; rows on 16-byte boundaries are read with the fewest instructions. */
+typedef struct ws_rows {
+  void* data;
+  uint64_t rows;
+  uint64_t inner;
+  int64_t stride_outer;
+  int64_t stride_inner;
+  uint64_t vocab;
+  int32_t dtype; /* WS_DTYPE_* */
+  int32_t reserved;
+} ws_rows;
+
+/* The k largest logits of every row by (logit descending, id ascending), as token
+ * ids and log-probabilities of softmax(x / temperature): ids and logprobs are
+ * [rows, k] without gaps. 1 <= k <= min(vocab, WS_TOP_MAX_K), temperature in [1e-6, 1e6].
+ * A logit of -inf has no place in a record: where a row has fewer than k others, the
+ * record ends with id -1 and log-probability -inf. A NaN logit is passed
+ * over too, and makes all log-probabilities of its row NaN, as +inf does. */
+WS_API int ws_top_logprobs(const ws_rows* logits, uint32_t k, float temperature, int64_t* ids, float* logprobs,
+                           int device, void* stream);
+
+/* How tokens are drawn. Each setting is one value for each row (`..._each`, device
+ * memory [rows]) or, where that is null, one value for all. */
+typedef struct ws_sampling {
+  const float* temperature_each;
+  const float* top_p_each;
+  const float* min_p_each;
+  const void* top_k_each; /* int32, or int64 with top_k_is_int64 */
+  int64_t top_k;
+  float temperature, top_p, min_p;
+  int32_t top_k_is_int64;
+} ws_sampling;
+
+/* Draws one token from every row with the given uniform number in [0, 1).
+ * With tokens ordered by (logit descending, id ascending) and
+ * w = exp((x - max x) / temperature), the tokens kept are a prefix of that order:
+ *   top_k >= 1: its first top_k (top_k <= 0: all);
+ *   top_p < 1: of these, those before which less than top_p of their weight lies
+ *     (at least the first; top_p <= 0 or NaN: the first alone);
+ *   min_p > 0: of these, those with w >= min_p (above 1 it counts as 1).
+ * The token is the first one, by id, whose cumulative weight among those kept is
+ * above uniform times their total. Borders are decided in 64 bits: weights are rounded to
+ * multiples of 2^-42 of the largest and summed exactly, so a result depends on no order of
+ * summation. temperature <= 0 or NaN: the first token of the order, as
+ * at temperature 1. tokens[r] = -1 for a row without a logit above -inf; NaN
+ * logits are never drawn; +inf logits share the weight. logprobs[r] (optional):
+ * the token's log-probability under softmax(x / temperature) of the whole row (NaN where the row holds a NaN
+ * or +inf). */
+WS_API int ws_sample(const ws_rows* logits, const float* uniform, const ws_sampling* sampling, int64_t* tokens,
+                     float* logprobs, int device, void* stream);
+
+/* A teacher's record for each row, as ws_top_logprobs writes it: `k` token ids and
+ * their log-probabilities, both [rows, k] without gaps. An entry whose id lies outside
+ * [0, vocab) or whose log-probability is -inf carries no mass; a token that
+ * comes twice counts twice. */
+#define WS_TAIL_DROP 0        /* the record's own probabilities: what lies outside it is left out */
+#define WS_TAIL_RENORMALIZE 1 /* its probabilities divided by their sum */
+typedef struct ws_teacher {
+  const void* ids;       /* int64 (ids_are_int32 == 0) or int32 */
+  const float* logprobs;
+  const float* weights;  /* [rows], or null: 1 for each row. A row of weight 0 is not read */
+  uint32_t k;            /* 1 .. WS_TOP_MAX_K */
+  int32_t ids_are_int32;
+  int32_t tail;          /* WS_TAIL_* */
+  float temperature;     /* of the student's softmax, > 0 */
+} ws_teacher;
+
+/* The loss of every row against its record, with q the record's probabilities,
+ * Q their sum, p = softmax(x / temperature) and w the row's weight:
+ *   loss = w * sum_j q_j (log q_j - log p[id_j])
+ * `stats` receives WS_DISTILL_STATS floats a row for ws_distill_backward. A row of
+ * weight 0 or whose record carries no mass has loss 0; a token of the record whose
+ * logit is -inf makes the loss +inf. */
+#define WS_DISTILL_STATS 2
+WS_API int ws_distill_forward(const ws_rows* logits, const ws_teacher* teacher, float* loss, float* stats, int device,
+                              void* stream);
+
+/* The loss's gradient with respect to the logits:
+ *   grad[i] = g w / temperature * (Q p[i] - sum of q_j over the j with id_j = i)
+ * rounded once to the logits' type. `stats` is the forward call's;
+ * `grad_loss` holds g of row r at (r / inner) * grad_outer + (r % inner) * grad_inner
+ * with the `inner` of `logits` (strides 0: one g for all rows). `grad` has the rows,
+ * vocabulary and type of `logits`; its rows must not overlap each other or the logits.
+ * A row of weight 0, or one without any finite logit, gets zeros. */
+WS_API int ws_distill_backward(const ws_rows* logits, const ws_teacher* teacher, const float* stats,
+                               const float* grad_loss, int64_t grad_outer, int64_t grad_inner, const ws_rows* grad,
+                               int device, void* stream);
+
+/* Both in one launch, for g = 1: the logits come from HBM once. */
+WS_API int ws_distill_step(const ws_rows* logits, const ws_teacher* teacher, float* loss, const ws_rows* grad,
+                           int device, void* stream);
+
 /* Frees host and device resources (delta.py relies on GC for the same), after
  * waiting for an apply still in flight. */
 WS_API void ws_plan_destroy(ws_plan* plan);

@@ -93,6 +93,50 @@ class PlanView(ctypes.Structure):
     ]
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [
+        ("data", P),
+        ("rows", u64),
+        ("inner", u64),
+        ("stride_outer", i64),
+        ("stride_inner", i64),
+        ("vocab", u64),
+        ("dtype", i32),
+        ("reserved", i32),
+    ]
+
+
+class Teacher(ctypes.Structure):
+    _fields_ = [
+        ("ids", P),
+        ("logprobs", P),
+        ("weights", P),
+        ("k", u32),
+        ("ids_are_int32", i32),
+        ("tail", i32),
+        ("temperature", ctypes.c_float),
+    ]
+
+
+class Sampling(ctypes.Structure):
+    _fields_ = [
+        ("temperature_each", P),
+        ("top_p_each", P),
+        ("min_p_each", P),
+        ("top_k_each", P),
+        ("top_k", i64),
+        ("temperature", ctypes.c_float),
+        ("top_p", ctypes.c_float),
+        ("min_p", ctypes.c_float),
+        ("top_k_is_int64", i32),
+    ]
+
+
+WS_TOP_MAX_K = 256
+WS_MAX_VOCAB = 1 << 20
+WS_DISTILL_STATS = 2
+TAILS = {"drop": 0, "renormalize": 1}
+
 # Every symbol declared in include/warpshift_b200.h, with its ctypes signature.
 SIGNATURES = {
     "ws_version": ([], ctypes.c_int),
@@ -111,6 +155,11 @@ SIGNATURES = {
     "ws_plan_save": ([P, ctypes.c_char_p], ctypes.c_int),
     "ws_plan_load": ([ctypes.c_char_p, ctypes.POINTER(TensorDesc), u64, ctypes.POINTER(BuildOptions), ctypes.POINTER(P)], ctypes.c_int),
     "ws_selftest_wait_timeout": ([u32, ctypes.c_int, P, ctypes.POINTER(u32)], ctypes.c_int),
+    "ws_top_logprobs": ([ctypes.POINTER(Rows), u32, ctypes.c_float, P, P, ctypes.c_int, P], ctypes.c_int),
+    "ws_sample": ([ctypes.POINTER(Rows), P, ctypes.POINTER(Sampling), P, P, ctypes.c_int, P], ctypes.c_int),
+    "ws_distill_forward": ([ctypes.POINTER(Rows), ctypes.POINTER(Teacher), P, P, ctypes.c_int, P], ctypes.c_int),
+    "ws_distill_backward": ([ctypes.POINTER(Rows), ctypes.POINTER(Teacher), P, P, i64, i64, ctypes.POINTER(Rows), ctypes.c_int, P], ctypes.c_int),
+    "ws_distill_step": ([ctypes.POINTER(Rows), ctypes.POINTER(Teacher), P, ctypes.POINTER(Rows), ctypes.c_int, P], ctypes.c_int),
     "ws_tensor_hashes": ([ctypes.POINTER(P), ctypes.POINTER(u64), u64, ctypes.c_int, P, ctypes.POINTER(u64)], ctypes.c_int),
 }
 WS_NOALLOC_MAX_TILES = 16384
