@@ -130,26 +130,39 @@ __device__ __forceinline__ void write_grad(const Record& r, uint32_t row, const 
   const bool none = a == 0.f && b == 0.f;
   T* out = grad - walk.head;  // by aligned position
   const bool same = (((uintptr_t)out) & 15u) == 0;
-  for (uint32_t u = first + threadIdx.x; u < last; u += kRowThreads) {
-    float f[kUnit];
-    if (none) {
+  const uint64_t nm = pair(-m, -m), cc = pair(r.c, r.c), aa = pair(a, a);
+  Batch<T> next;
+  if (none) next = Batch<T>{};
+  else if (first < last) next.load(walk, first, last);
+  for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
+    const Batch<T> now = next;
+    if (!none && u0 + Batch<T>::kSpan < last) next.load(walk, u0 + Batch<T>::kSpan, last);
 #pragma unroll
-      for (uint32_t i = 0; i < kUnit; ++i) f[i] = 0.f;
-    } else {
-      walk.load(u, f);
+    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+      const uint32_t u = u0 + j * kRowThreads + threadIdx.x;
+      if (u >= last) continue;
+      float f[kUnit];
+      unpack<T>(now.raw[j], f);
+      if (!none) {
 #pragma unroll
-      for (uint32_t i = 0; i < kUnit; ++i) f[i] = a * ex2((f[i] - m) * r.c);
-    }
-    if (same && walk.whole(u)) {
-      const Raw<T> w = pack<T>(f);
-      uint4* v = reinterpret_cast<uint4*>(out + (size_t)u * kUnit);
+        for (uint32_t i = 0; i < kUnit; i += 2) {
+          const float2 e = unpair(mul2(add2(pair(f[i], f[i + 1]), nm), cc));
+          const float2 g = unpair(mul2(aa, pair(ex2(e.x), ex2(e.y))));
+          f[i] = g.x;
+          f[i + 1] = g.y;
+        }
+      }
+      if (same && walk.whole(u)) {
+        const Raw<T> w = pack<T>(f);
+        uint4* v = reinterpret_cast<uint4*>(out + (size_t)u * kUnit);
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof(T) / 2); ++i) v[i] = w.v[i];
-    } else {
+        for (uint32_t i = 0; i < sizeof(T) / 2; ++i) v[i] = w.v[i];
+      } else {
 #pragma unroll
-      for (uint32_t i = 0; i < kUnit; ++i) {
-        const uint32_t p = u * kUnit + i;
-        if (p >= walk.head && p < walk.end) out[p] = from_float<T>(f[i]);
+        for (uint32_t i = 0; i < kUnit; ++i) {
+          const uint32_t p = u * kUnit + i;
+          if (p >= walk.head && p < walk.end) out[p] = from_float<T>(f[i]);
+        }
       }
     }
   }
@@ -174,13 +187,6 @@ __device__ __forceinline__ void write_grad(const Record& r, uint32_t row, const 
   }
 }
 
-// Units of the row that block `rank` of `blocks` walks.
-__device__ __forceinline__ void split_units(uint32_t units, uint32_t rank, uint32_t blocks, uint32_t& first, uint32_t& last) {
-  const uint32_t each = (units + blocks - 1) / blocks;
-  first = min(rank * each, units);
-  last = min(first + each, units);
-}
-
 template <class T>
 __global__ void __launch_bounds__(kRowThreads)
     distill_forward_kernel(RowSet x, Record r, float* __restrict__ loss, float* __restrict__ stats) {
@@ -202,13 +208,7 @@ __global__ void __launch_bounds__(kRowThreads)
   const RowWalk<T> walk(src, x.vocab);
   uint32_t first, last;
   split_units(walk.units, rank, blocks, first, last);
-  Soft soft;
-  for (uint32_t u = first + threadIdx.x; u < last; u += kRowThreads) {
-    float f[kUnit];
-    walk.load(u, f);
-    soft.add(f, r.c);
-  }
-  soft = cluster_soft(block_soft(soft, r.c, soft_scratch), r.c, &mine);
+  const Soft soft = cluster_soft(row_soft(walk, first, last, r.c, soft_scratch), r.c, &mine);
   if (rank == 0) {
     const RecordSums t = record_sums<T>(r, row, src, x.vocab, soft.m, sums);
     if (threadIdx.x == 0) {
@@ -223,11 +223,12 @@ __global__ void __launch_bounds__(kRowThreads)
 template <class T>
 __global__ void __launch_bounds__(kRowThreads)
     distill_backward_kernel(RowSet x, Record r, const float* __restrict__ stats, const float* __restrict__ grad_loss,
-                            int64_t grad_outer, int64_t grad_inner, RowSet dx, uint32_t pieces) {
+                            int64_t grad_outer, int64_t grad_inner, RowSet dx) {
   __shared__ int ids[kRowThreads];
   __shared__ float qs[kRowThreads];
   __shared__ double sums[kRowWarps];
-  const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t pieces = cluster.num_blocks(), piece = cluster.block_rank(), row = blockIdx.x / pieces;
   const float w = r.weights ? r.weights[row] : 1.f;
   const float2 st = reinterpret_cast<const float2*>(stats)[row];
   const uint32_t o = row / x.inner, in = row - o * x.inner;
@@ -268,13 +269,7 @@ __global__ void __launch_bounds__(kRowThreads)
   split_units(walk.units, rank, blocks, first, last);
   float m = 0.f, shift = 0.f, a = 0.f, b = 0.f, l = 0.f;
   if (w != 0.f) {  // the same for the whole cluster
-    Soft soft;
-    for (uint32_t u = first + threadIdx.x; u < last; u += kRowThreads) {
-      float f[kUnit];
-      walk.load(u, f);
-      soft.add(f, r.c);
-    }
-    soft = cluster_soft(block_soft(soft, r.c, soft_scratch), r.c, &mine);
+    const Soft soft = cluster_soft(row_soft(walk, first, last, r.c, soft_scratch), r.c, &mine);
     const RecordSums t = record_sums<T>(r, row, src, x.vocab, soft.m, sums);
     RowGrad g;
     l = w * finish_loss(r, t, soft, g);
@@ -338,7 +333,7 @@ extern "C" int ws_distill_forward(const ws_rows* logits, const ws_teacher* teach
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(distill_forward_kernel<T>, (uint64_t)x.rows, 1, 0, stream, x.set, r, loss, stats);
+        return launch_rows(distill_forward_kernel<T>, x.rows, blocks_a_row(x.rows, x.set.vocab / kUnit), stream, x.set, r, loss, stats);
       });
     return done(e, "distill forward");
   });
@@ -358,13 +353,13 @@ extern "C" int ws_distill_backward(const ws_rows* logits, const ws_teacher* teac
     if (x.rows == 0) return (int)WS_OK;
     if (!stats || !grad_loss) return fail(WS_ERR_INVALID, "null pointer");
     if ((uintptr_t)stats % 8) return fail(WS_ERR_INVALID, "stats must be 8-byte aligned");
+    const uint32_t pieces = blocks_a_row(x.rows, x.set.vocab / kUnit);
     DeviceGuard guard(device);
     cudaError_t e = guard.error();
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(distill_backward_kernel<T>, (uint64_t)x.rows, 1, 0, stream, x.set, r, stats, grad_loss, grad_outer,
-                           grad_inner, dx.set, 1u);
+        return launch_rows(distill_backward_kernel<T>, x.rows, pieces, stream, x.set, r, stats, grad_loss, grad_outer, grad_inner, dx.set);
       });
     return done(e, "distill backward");
   });
@@ -387,7 +382,7 @@ extern "C" int ws_distill_step(const ws_rows* logits, const ws_teacher* teacher,
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(distill_step_kernel<T>, (uint64_t)x.rows, 1, 0, stream, x.set, r, loss, dx.set);
+        return launch_rows(distill_step_kernel<T>, x.rows, blocks_a_row(x.rows, x.set.vocab / kUnit), stream, x.set, r, loss, dx.set);
       });
     return done(e, "distill step");
   });

@@ -1,4 +1,5 @@
 // What a row of logits answers: its top log-probabilities, and a token drawn from it.
+#include <cfloat>
 #include <string>
 
 #include "ws_guard.h"
@@ -14,22 +15,36 @@ namespace cg = cooperative_groups;
 // One pass over the row gives its maximum m and S = sum exp((x - m) / t), and keeps
 // the candidates for the k largest logits in shared memory: a candidate is 64 bits, the order key
 // of its logit above the complement of its id, so that no two are equal and the
-// larger one comes first in the record. A step takes one unit of 8 logits from each
-// thread; those above the k-th largest candidate so far are appended, at most 2048 of them, and
-// when more than k are there, all but the k largest are dropped.
+// larger one comes first in the record.
+//
+// What a logit costs is one comparison of its unit's maximum with a threshold, below which nothing can be in
+// the record. The threshold comes from maxima that are at hand anyway: every thread keeps the maximum of each
+// of its kUnits places in a step over all steps, kRowThreads * kUnits logits of different
+// ids, the k-th largest of which is a lower bound of the k-th largest logit, and a close one. It is
+// found by bisection over the upper 16 bits of the order keys after steps 1, 2, 4, 8, ...
+// and at the end, when the list holds few more than k candidates.
+//
+// The list has room for k candidates and all of a step's that one unit of each thread
+// gives. A step that would overflow it (ascending or equal logits) is taken again unit
+// by unit, dropping all but the k largest before each: slow, and right for any row.
 constexpr uint32_t kCandidates = WS_TOP_MAX_K + kRowThreads * kUnit;
+constexpr uint32_t kSorted = 512;  // candidates that are put in order by counting
 
 struct TopShared {
   uint64_t list[kCandidates];
-  uint32_t count;
+  uint64_t sorted[WS_TOP_MAX_K];  // the block's k largest in order, for the other blocks of the cluster
+  uint32_t count, sorted_count;
   uint32_t sums[kRowWarps];
+  uint2 votes[2][kRowWarps];
   float2 soft[kRowWarps];
+  float2 soft_mine;
 };
 
 __device__ __forceinline__ uint64_t candidate(float x, uint32_t id) { return ((uint64_t)order_key(x) << 32) | (0xFFFFFFFFu - id); }
+__device__ __forceinline__ float candidate_value(uint64_t v) { return key_value((uint32_t)(v >> 32)); }
 
 // Keeps the k largest of s.list's first n > k candidates (in no order) and returns the smallest of these.
-__device__ uint64_t keep_largest(TopShared& s, uint32_t n, uint32_t k) {
+__device__ __noinline__ uint64_t keep_largest(TopShared& s, uint32_t n, uint32_t k) {
   constexpr uint32_t kMine = (kCandidates + kRowThreads - 1) / kRowThreads;
   uint64_t mine[kMine];
 #pragma unroll
@@ -54,51 +69,194 @@ __device__ uint64_t keep_largest(TopShared& s, uint32_t n, uint32_t k) {
   return edge;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kRowThreads)
-    top_kernel(RowSet x, uint32_t k, float c, float inv_t, int64_t* __restrict__ ids, float* __restrict__ logprobs) {
-  __shared__ TopShared s;
-  const uint32_t row = blockIdx.x;
-  const RowWalk<T> walk(row_ptr<T>(x, row), x.vocab);
-  if (threadIdx.x == 0) s.count = 0;
-  __syncthreads();
-  Soft soft;
-  uint64_t edge = 0;  // candidates not above it are of no use
-  for (uint32_t u0 = 0; u0 < walk.units; u0 += kRowThreads) {
-    const uint32_t u = u0 + threadIdx.x;
-    if (u < walk.units) {
-      float f[kUnit];
-      walk.load(u, f);
-      soft.add(f, c);
+// A logit that at least k of the block's maxima reach, as large as 16 bits of its order key
+// tell; the lowest finite number where fewer than k are above -inf. Two bits a round: the
+// counts of three trials by one shuffle-free reduction in the warp, and one barrier.
+template <uint32_t N>
+__device__ __forceinline__ float kth_of_maxima(TopShared& s, const float (&top)[N], uint32_t k) {
+  uint32_t key[N];
 #pragma unroll
-      for (uint32_t i = 0; i < kUnit; ++i) {
-        if (f[i] > -INFINITY) {
-          const uint64_t v = candidate(f[i], u * kUnit + i - walk.head);
-          if (v > edge) s.list[atomicAdd(&s.count, 1u)] = v;
+  for (uint32_t j = 0; j < N; ++j) key[j] = order_key(top[j]) >> 16;
+  uint32_t edge = 0;
+#pragma unroll
+  for (int bit = 14; bit >= 0; bit -= 2) {
+    uint32_t low = 0, high = 0;  // counts of trials 1 and 2, and of trial 3
+#pragma unroll
+    for (uint32_t j = 0; j < N; ++j) {
+      low += (key[j] >= (edge | (1u << bit)) ? 1u : 0u) + (key[j] >= (edge | (2u << bit)) ? 0x10000u : 0u);
+      high += key[j] >= (edge | (3u << bit)) ? 1u : 0u;
+    }
+    low = __reduce_add_sync(0xFFFFFFFFu, low);
+    high = __reduce_add_sync(0xFFFFFFFFu, high);
+    uint2* votes = s.votes[(bit >> 1) & 1];  // the other half may still be read
+    if ((threadIdx.x & 31u) == 0) votes[threadIdx.x >> 5] = make_uint2(low, high);
+    __syncthreads();
+    low = high = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kRowWarps; ++w) {
+      low += votes[w].x;
+      high += votes[w].y;
+    }
+    const uint32_t step = high >= k ? 3u : (low >> 16) >= k ? 2u : (low & 0xFFFFu) >= k ? 1u : 0u;
+    edge |= step << bit;
+  }
+  constexpr uint32_t kNone = 0x007Fu;  // upper half of -inf's key
+  return edge <= kNone ? -FLT_MAX : key_value(edge << 16);
+}
+
+// The statistics and the k largest logits of units [first, last) of a row: s.sorted_count (at most k) candidates in s.sorted, in
+// order. Every thread gets the statistics.
+template <class T>
+__device__ __forceinline__ Soft row_top(const RowWalk<T>& walk, uint32_t first, uint32_t last, float c, uint32_t k, TopShared& s) {
+  using B = Batch<T>;
+  if (threadIdx.x == 0) s.count = 0;
+  Soft soft;
+  float most[B::kUnits];
+#pragma unroll
+  for (uint32_t j = 0; j < B::kUnits; ++j) most[j] = -INFINITY;
+  float edge = -FLT_MAX;  // logits below it are of no use; nor are -inf and NaN
+  B next;
+  if (first < last) next.load(walk, first, last);
+  __syncthreads();
+  uint32_t step = 1;
+  for (uint32_t u0 = first; u0 < last; u0 += B::kSpan, ++step) {
+    const B now = next;
+    if (u0 + B::kSpan < last) next.load(walk, u0 + B::kSpan, last);
+    float top[B::kUnits], all = -INFINITY;
+#pragma unroll
+    for (uint32_t j = 0; j < B::kUnits; ++j) {
+      top[j] = unit_max<T>(now.raw[j]);
+      most[j] = fmaxf(most[j], top[j]);
+      all = fmaxf(all, top[j]);
+    }
+    soft.add(now, all, c);
+    if ((step & (step - 1)) == 0) edge = fmaxf(edge, kth_of_maxima(s, most, k));
+    const uint32_t before = s.count;
+    __syncthreads();  // everyone has it
+    if (all >= edge) {
+#pragma unroll
+      for (uint32_t j = 0; j < B::kUnits; ++j) {
+        if (top[j] >= edge) {
+          float f[kUnit];
+          unpack<T>(now.raw[j], f);
+          const uint32_t id = (u0 + j * kRowThreads + threadIdx.x) * kUnit - walk.head;
+#pragma unroll
+          for (uint32_t i = 0; i < kUnit; ++i) {
+            if (f[i] >= edge) {
+              const uint32_t at = atomicAdd(&s.count, 1u);
+              if (at < kCandidates) s.list[at] = candidate(f[i], id + i);
+            }
+          }
         }
       }
     }
     __syncthreads();
-    if (s.count > k) edge = keep_largest(s, s.count, k);
-    __syncthreads();
-  }
-  soft = block_soft(soft, c, s.soft);
-  const uint32_t n = s.count;
-  const float log_s = (float)log((double)soft.s);
-  if (threadIdx.x < k) {
-    const size_t out = (size_t)row * k;
-    if (threadIdx.x < n) {
-      const uint64_t v = s.list[threadIdx.x];
-      uint32_t place = 0;
-      for (uint32_t i = 0; i < n; ++i) place += s.list[i] > v;
-      const float d = (float)(((double)key_value((uint32_t)(v >> 32)) - (double)soft.m) * (double)inv_t);
-      ids[out + place] = (int64_t)(0xFFFFFFFFu - (uint32_t)v);
-      logprobs[out + place] = d - log_s;
-    } else {
-      ids[out + threadIdx.x] = -1;
-      logprobs[out + threadIdx.x] = isnan(soft.s) ? NAN : -INFINITY;
+    if (s.count > kCandidates) {
+      __syncthreads();
+      if (threadIdx.x == 0) s.count = before;
+      __syncthreads();
+      uint64_t least = 0;
+      for (uint32_t j = 0; j < B::kUnits; ++j) {
+        if (s.count > k) least = keep_largest(s, s.count, k);
+        __syncthreads();
+        Raw<T> raw = now.raw[0];
+#pragma unroll
+        for (uint32_t q = 1; q < B::kUnits; ++q)
+          if (q == j) raw = now.raw[q];
+        float f[kUnit];
+        unpack<T>(raw, f);
+        const uint32_t id = (u0 + j * kRowThreads + threadIdx.x) * kUnit - walk.head;
+#pragma unroll
+        for (uint32_t i = 0; i < kUnit; ++i) {
+          if (f[i] >= edge) {
+            const uint64_t v = candidate(f[i], id + i);
+            if (v > least) s.list[atomicAdd(&s.count, 1u)] = v;
+          }
+        }
+        __syncthreads();
+      }
+      if (s.count > k) least = keep_largest(s, s.count, k);
+      edge = fmaxf(edge, least ? candidate_value(least) : -FLT_MAX);
+      __syncthreads();
     }
   }
+  // Of the candidates those that reach the last threshold, in order. A thread holds at most kMine of them.
+  edge = fmaxf(edge, kth_of_maxima(s, most, k));
+  constexpr uint32_t kMine = (kCandidates + kRowThreads - 1) / kRowThreads;
+  uint64_t mine[kMine];
+  const uint32_t found = s.count;
+#pragma unroll
+  for (uint32_t i = 0; i < kMine; ++i) {
+    const uint32_t at = i * kRowThreads + threadIdx.x;
+    mine[i] = at < found ? s.list[at] : 0;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < kMine; ++i)
+    if (mine[i] && candidate_value(mine[i]) >= edge) s.list[atomicAdd(&s.count, 1u)] = mine[i];
+  __syncthreads();
+  if (s.count > kSorted) keep_largest(s, s.count, k);  // k <= WS_TOP_MAX_K <= kSorted remain
+  const uint32_t n = s.count;
+  if (threadIdx.x == 0) s.sorted_count = min(n, k);
+  for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) {
+    const uint64_t v = s.list[i];
+    uint32_t place = 0;
+#pragma unroll 4
+    for (uint32_t q = 0; q < n; ++q) place += s.list[q] > v;
+    if (place < k) s.sorted[place] = v;
+  }
+  return block_soft(soft, c, s.soft);  // with a barrier behind s.sorted
+}
+
+// The cluster's record: place of this block's i-th candidate, which is i and how many of the other blocks' are larger.
+__device__ __forceinline__ uint32_t cluster_place(TopShared& s, uint32_t i, uint64_t v) {
+  cg::cluster_group cluster = cg::this_cluster();
+  uint32_t place = i;
+  for (uint32_t b = 0; b < cluster.num_blocks(); ++b) {
+    if (b == cluster.block_rank()) continue;
+    const TopShared* o = cluster.map_shared_rank(&s, b);
+    uint32_t lo = 0, hi = o->sorted_count;
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (o->sorted[mid] > v) lo = mid + 1;
+      else hi = mid;
+    }
+    place += lo;
+  }
+  return place;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kRowThreads, 3)
+    top_kernel(RowSet x, uint32_t k, float c, float inv_t, int64_t* __restrict__ ids, float* __restrict__ logprobs) {
+  __shared__ TopShared s;
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / blocks;
+  const RowWalk<T> walk(row_ptr<T>(x, row), x.vocab);
+  uint32_t first, last;
+  split_units(walk.units, rank, blocks, first, last);
+  const Soft soft = cluster_soft(row_top(walk, first, last, c, k, s), c, &s.soft_mine);
+  const double log_s = log((double)soft.s);
+  const size_t out = (size_t)row * k;
+  if (threadIdx.x < s.sorted_count) {
+    const uint64_t v = s.sorted[threadIdx.x];
+    const uint32_t place = blocks > 1 ? cluster_place(s, threadIdx.x, v) : threadIdx.x;
+    if (place < k) {
+      ids[out + place] = (int64_t)(0xFFFFFFFFu - (uint32_t)v);
+      logprobs[out + place] = (float)(((double)candidate_value(v) - (double)soft.m) * (double)inv_t - log_s);
+    }
+  }
+  if (rank == 0) {
+    uint32_t n = 0;
+    for (uint32_t b = 0; b < blocks; ++b) n += cluster.map_shared_rank(&s, b)->sorted_count;
+    for (uint32_t i = n + threadIdx.x; i < k; i += kRowThreads) {
+      ids[out + i] = -1;
+      logprobs[out + i] = isnan(soft.s) ? NAN : -INFINITY;
+    }
+  }
+  if (blocks > 1) cluster.sync();  // the blocks' shared memory is read until here
 }
 
 // ------------------------------------------------------------ sampling
@@ -339,13 +497,7 @@ __global__ void __launch_bounds__(kRowThreads)
   const uint32_t each = (chunks + blocks - 1) / blocks;
   const uint32_t chunk0 = min(rank * each, chunks), chunk1 = min(chunk0 + each, chunks);
   SampleRow<T> row{walk, min(chunk0 * kChunkUnits, walk.units), min(chunk1 * kChunkUnits, walk.units), 0.f, 1.0 / (double)t};
-  Soft soft;
-  for (uint32_t u = row.first + threadIdx.x; u < row.last; u += kRowThreads) {
-    float f[kUnit];
-    walk.load(u, f);
-    soft.add(f, c);
-  }
-  soft = cluster_soft(block_soft(soft, c, s.soft_scratch), c, &s.soft_mine);
+  const Soft soft = cluster_soft(row_soft(walk, row.first, row.last, c, s.soft_scratch), c, &s.soft_mine);
   row.m = soft.m;
   if (soft.m == -INFINITY) {  // the same for the whole cluster
     if (rank == 0 && threadIdx.x == 0 && logprobs) logprobs[r] = isnan(soft.s) ? NAN : -INFINITY;
@@ -488,7 +640,7 @@ __global__ void __launch_bounds__(kRowThreads)
       if (hit) {
         if (lane == (uint32_t)(__ffs(hit) - 1)) {
           tokens[r] = (int64_t)(p - walk.head);
-          if (logprobs) logprobs[r] = (float)(((double)v - (double)soft.m) * row.inv_t) - (float)log((double)soft.s);
+          if (logprobs) logprobs[r] = (float)(((double)v - (double)soft.m) * row.inv_t - log((double)soft.s));
         }
         break;
       }
@@ -529,7 +681,7 @@ extern "C" int ws_top_logprobs(const ws_rows* logits, uint32_t k, float temperat
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(top_kernel<T>, (uint64_t)x.rows, 1, 0, stream, x.set, k, kLog2e / temperature, 1.f / temperature, ids,
+        return launch_rows(top_kernel<T>, x.rows, blocks_a_row(x.rows, x.set.vocab / kUnit), stream, x.set, k, kLog2e / temperature, 1.f / temperature, ids,
                            logprobs);
       });
     return done(e, "top log-probabilities");
@@ -551,7 +703,7 @@ extern "C" int ws_sample(const ws_rows* logits, const float* uniform, const ws_s
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(sample_kernel<T>, (uint64_t)x.rows, 1, 0, stream, x.set, uniform, *sampling, tokens, logprobs);
+        return launch_rows(sample_kernel<T>, x.rows, blocks_a_row(x.rows, x.set.vocab / kUnit), stream, x.set, uniform, *sampling, tokens, logprobs);
       });
     return done(e, "sample");
   });

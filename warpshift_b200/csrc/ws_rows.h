@@ -154,6 +154,87 @@ struct RowWalk {
   }
 };
 
+// 16 bytes that are read once: not kept in L1.
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// -inf in every element of a word.
+template <class T>
+constexpr uint32_t kNegInf = 0xFF800000u;
+template <>
+constexpr uint32_t kNegInf<__nv_bfloat16> = 0xFF80FF80u;
+template <>
+constexpr uint32_t kNegInf<__half> = 0xFC00FC00u;
+
+// What a block reads of a row in one step: kBatch units from each thread, thread t's j-th one at
+// u0 + j * kRowThreads + t. 64 bytes a thread in flight for either element size.
+template <class T>
+struct Batch {
+  static constexpr uint32_t kUnits = 8 / sizeof(T);
+  static constexpr uint32_t kSpan = kUnits * kRowThreads;  // units of the block's step
+  Raw<T> raw[kUnits];
+
+  // Units [u0, u0 + kSpan) up to `last`; what lies outside is -inf.
+  __device__ __forceinline__ void load(const RowWalk<T>& walk, uint32_t u0, uint32_t last) {
+    if (u0 * kUnit >= walk.head && u0 + kSpan <= last && (u0 + kSpan) * kUnit <= walk.end) {
+      const T* p = walk.aligned + (size_t)(u0 + threadIdx.x) * kUnit;
+#pragma unroll
+      for (uint32_t j = 0; j < kUnits; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(T) / 2; ++i) raw[j].v[i] = load16(p + j * kRowThreads * kUnit + i * (16 / sizeof(T)));
+      return;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kUnits; ++j) {
+      const uint32_t u = u0 + j * kRowThreads + threadIdx.x;
+      if (u < last && walk.whole(u)) {
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(T) / 2; ++i)
+          raw[j].v[i] = load16(walk.aligned + (size_t)u * kUnit + i * (16 / sizeof(T)));
+      } else {
+        float f[kUnit];
+#pragma unroll
+        for (uint32_t i = 0; i < kUnit; ++i) {
+          const uint32_t p = u * kUnit + i;
+          f[i] = u < last && p >= walk.head && p < walk.end ? walk.at(p) : -INFINITY;
+        }
+        raw[j] = pack<T>(f);
+      }
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (uint32_t j = 0; j < kUnits; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < sizeof(T) / 2; ++i) raw[j].v[i] = make_uint4(kNegInf<T>, kNegInf<T>, kNegInf<T>, kNegInf<T>);
+  }
+};
+
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+
 // Running maximum m and sum s of 2^((x - m) c), c = log2(e) / temperature. The
 // difference x - m is taken before the product, so logits of any size (a mask of
 // the type's lowest value, say) give exponents that are exact near the maximum.
@@ -161,17 +242,29 @@ struct RowWalk {
 struct Soft {
   float m = -INFINITY, s = 0.f;
 
-  __device__ __forceinline__ void add(const float (&f)[kUnit], float c) {
-    float top = f[0];
-#pragma unroll
-    for (uint32_t i = 1; i < kUnit; ++i) top = fmaxf(top, f[i]);
+  // One step's logits, of which `top` is the largest. They are added up among themselves first, which
+  // keeps the chains of additions short.
+  template <class T>
+  __device__ __forceinline__ void add(const Batch<T>& b, float top, float c) {
     if (top > m) {
       s *= ex2((m - top) * c);
       m = top;
     }
     const float base = m == -INFINITY ? 0.f : m;
+    const uint64_t nb = pair(-base, -base), cc = pair(c, c);
+    uint64_t sum = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kUnit; ++i) s += ex2((f[i] - base) * c);
+    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+      float f[kUnit];
+      unpack<T>(b.raw[j], f);
+#pragma unroll
+      for (uint32_t i = 0; i < kUnit; i += 2) {
+        const float2 e = unpair(mul2(add2(pair(f[i], f[i + 1]), nb), cc));
+        sum = add2(sum, pair(ex2(e.x), ex2(e.y)));
+      }
+    }
+    const float2 t = unpair(sum);
+    s += t.x + t.y;
   }
   __device__ __forceinline__ void merge(float m2, float s2, float c) {
     const float top = fmaxf(m, m2);
@@ -247,6 +340,31 @@ __device__ __forceinline__ Soft cluster_soft(const Soft& block, float c, float2*
   return r;
 }
 
+template <class T>
+__device__ __forceinline__ float unit_max(const Raw<T>& r) {
+  float f[kUnit];
+  unpack<T>(r, f);
+  return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+}
+
+// Statistics of units [first, last) of a row, for the whole block. The loads of a step are in flight while
+// the step before is summed up.
+template <class T>
+__device__ __forceinline__ Soft row_soft(const RowWalk<T>& walk, uint32_t first, uint32_t last, float c, float2* scratch) {
+  Soft soft;
+  Batch<T> next;
+  if (first < last) next.load(walk, first, last);
+  for (uint32_t u = first; u < last; u += Batch<T>::kSpan) {
+    const Batch<T> now = next;
+    if (u + Batch<T>::kSpan < last) next.load(walk, u + Batch<T>::kSpan, last);
+    float top = unit_max<T>(now.raw[0]);
+#pragma unroll
+    for (uint32_t j = 1; j < Batch<T>::kUnits; ++j) top = fmaxf(top, unit_max<T>(now.raw[j]));
+    soft.add(now, top, c);
+  }
+  return block_soft(soft, c, scratch);
+}
+
 // Floats as integers of the same order (-0 is taken as +0 first, so that equal
 // logits have equal keys).
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -255,6 +373,13 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+// Units of the row that block `rank` of `blocks` walks.
+__device__ __forceinline__ void split_units(uint32_t units, uint32_t rank, uint32_t blocks, uint32_t& first, uint32_t& last) {
+  const uint32_t each = (units + blocks - 1) / blocks;
+  first = min(rank * each, units);
+  last = min(first + each, units);
 }
 
 // ---------------------------------------------------------------- host side
@@ -300,13 +425,19 @@ cudaError_t by_type(int dtype, F&& f) {
   }
 }
 
-// Launches `blocks` blocks of kRowThreads threads in clusters of `cluster`.
+// How many blocks (a cluster: 1, 2, 4 or 8) share each of `rows` rows of `units` units.
+inline uint32_t blocks_a_row(uint32_t rows, uint32_t units) {
+  uint32_t c = 1;
+  while (c < 8 && (uint64_t)rows * c * 2 <= 592 && units / c >= 512) c *= 2;
+  return c;
+}
+
+// Launches `rows` clusters of `cluster` blocks of kRowThreads threads.
 template <class... P, class... A>
-cudaError_t launch_rows(void (*kernel)(P...), uint64_t blocks, uint32_t cluster, size_t smem, void* stream, A... args) {
+cudaError_t launch_rows(void (*kernel)(P...), uint32_t rows, uint32_t cluster, void* stream, A... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.gridDim = dim3(rows * cluster);
   cfg.blockDim = dim3(kRowThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeClusterDimension;
