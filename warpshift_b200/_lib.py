@@ -173,6 +173,8 @@ _lib: ctypes.CDLL | None = None
 def load() -> ctypes.CDLL:
     """Load the native library (raises RuntimeError if it has not been built)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not LIBRARY.exists():

@@ -58,229 +58,327 @@ struct Record {
   float inv_t;  // 1 / temperature
 };
 
-// Entry j of a row's record; a token id of -1 has no mass.
-__device__ __forceinline__ void record_entry(const Record& r, uint32_t row, uint32_t j, uint32_t vocab, int& id, float& lp) {
-  id = -1;
-  lp = -INFINITY;
-  if (j >= r.k) return;
-  const size_t at = (size_t)row * r.k + j;
-  const int64_t raw = r.ids32 ? ((const int32_t*)r.ids)[at] : ((const int64_t*)r.ids)[at];
-  lp = r.logprobs[at];
-  if (raw >= 0 && raw < (int64_t)vocab && lp > -INFINITY) id = (int)raw;
-}
+constexpr uint32_t kDepth = 3;      // steps in flight of the kernels that read a row once
+constexpr uint32_t kStepDepth = 4;  // of the one that reads it twice: a block's share up to 64 KiB stays
 
-// A row's record summed up. After renormalising, probabilities are taken relative to the
-// record's largest one (shift = its log-probability), so that a record far out in the teacher's
-// tail neither underflows nor overflows; shift is 0 otherwise.
-struct RecordSums {
-  double q, q_lp, q_d;  // sums of q, q lp and q (x - m) / t with q = exp(lp - shift)
-  float shift;
-};
+// Entry `threadIdx.x` of a row's record and the logit of its token; a token id of -1 has no mass.
+struct Entry {
+  int id = -1;
+  float lp = -INFINITY, x = 0.f;
 
-// What the gradient of a row needs: dense part mass_over_s * exp((x_i - m) / t), and q_scale * exp(lp - shift).
-struct RowGrad {
-  float m, mass_over_s, q_scale;
-};
-
-// Entry `threadIdx.x` of the record and the record's shift.
-__device__ __forceinline__ float record_shift(const Record& r, int id, float lp, float* scratch) {
-  if (!r.renormalize) return 0.f;
-  const float top = block_max(id >= 0 ? lp : -INFINITY, scratch);
-  return top == -INFINITY ? 0.f : top;
-}
-
-template <class T>
-__device__ __forceinline__ RecordSums record_sums(const Record& r, uint32_t row, const T* x, uint32_t vocab, float m,
-                                                  double* scratch) {
-  int id;
-  float lp;
-  record_entry(r, row, threadIdx.x, vocab, id, lp);
-  RecordSums t;
-  t.shift = record_shift(r, id, lp, reinterpret_cast<float*>(scratch));
-  double q = id >= 0 ? exp((double)lp - (double)t.shift) : 0.0, q_lp = 0.0, q_d = 0.0;
-  if (q != 0.0) {
-    q_lp = q * (double)lp;
-    q_d = q * (((double)to_float(x[id]) - (double)m) * (double)r.inv_t);
+  template <class T>
+  __device__ __forceinline__ void load(const Record& r, uint32_t row, const T* logits, uint32_t vocab) {
+    if (threadIdx.x >= r.k) return;
+    const size_t at = (size_t)row * r.k + threadIdx.x;
+    const int64_t raw = r.ids32 ? ((const int32_t*)r.ids)[at] : ((const int64_t*)r.ids)[at];
+    const float l = r.logprobs[at];
+    if (raw >= 0 && raw < (int64_t)vocab && l > -INFINITY) {
+      id = (int)raw;
+      lp = l;
+      x = to_float(logits[raw]);
+    }
   }
-  t.q = block_sum(q, scratch);
-  t.q_lp = block_sum(q_lp, scratch);
-  t.q_d = block_sum(q_d, scratch);
-  return t;
+};
+
+// A record summed up in 64 bits, by warps and then by one thread. Probabilities are taken relative to
+// the largest one where they are renormalised (shift = its log-probability, else 0), so that a record far out in
+// the teacher's tail neither underflows nor overflows, and logits relative to the largest one of the record, so that
+// nothing is lost where logits are huge (a mask of the type's lowest value).
+struct RecordSums {
+  double q = 0.0, q_lp = 0.0, q_x = 0.0;  // sums of q, q lp and q (x - at), q = exp(lp - shift)
+  float shift = 0.f, at = 0.f;
+
+  __device__ __forceinline__ void merge(const RecordSums& o) {
+    if (o.q == 0.0) return;
+    if (q == 0.0) {
+      *this = o;
+      return;
+    }
+    const float s = fmaxf(shift, o.shift);
+    const double mine = shift == s ? 1.0 : exp((double)shift - (double)s);
+    const double his = o.shift == s ? 1.0 : exp((double)o.shift - (double)s);
+    q_x = mine * q_x + his * (o.q_x + o.q * ((double)o.at - (double)at));
+    q = mine * q + his * o.q;
+    q_lp = mine * q_lp + his * o.q_lp;
+    shift = s;
+  }
+};
+
+// The warp's part of the record into `part` (one slot for each warp).
+__device__ __forceinline__ void sum_record(const Record& r, const Entry& e, RecordSums* part) {
+  const uint32_t warp = threadIdx.x >> 5;
+  RecordSums t;
+  if (warp * 32 < r.k) {
+    const uint32_t none = order_key(-INFINITY);
+    if (r.renormalize) {
+      const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, e.id >= 0 ? order_key(e.lp) : none);
+      t.shift = top == none ? 0.f : key_value(top);
+    }
+    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, e.id >= 0 && e.x > -INFINITY ? order_key(e.x) : none);
+    t.at = top == none ? 0.f : key_value(top);
+    t.q = e.id >= 0 ? exp((double)e.lp - (double)t.shift) : 0.0;
+    if (t.q != 0.0) {
+      t.q_lp = t.q * (double)e.lp;
+      t.q_x = t.q * ((double)e.x - (double)t.at);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      t.q += __shfl_xor_sync(0xFFFFFFFFu, t.q, o);
+      t.q_lp += __shfl_xor_sync(0xFFFFFFFFu, t.q_lp, o);
+      t.q_x += __shfl_xor_sync(0xFFFFFFFFu, t.q_x, o);
+    }
+  }
+  if ((threadIdx.x & 31u) == 0) part[warp] = t;
 }
 
-// The row's loss before its weight, and the gradient's factors (0: no gradient).
-__device__ __forceinline__ float finish_loss(const Record& r, const RecordSums& t, const Soft& soft, RowGrad& g) {
-  g = RowGrad{soft.m, 0.f, 0.f};
-  if (t.q == 0.0) return 0.f;                  // no mass on record
-  if (soft.m == -INFINITY) return INFINITY;    // no finite logit
+// What the gradient of a row needs: (mass / S) exp((x_i - m) / t) for the dense part, scale exp(lp - shift) for
+// the record's. Both 0: the row has no gradient, and its logits are not read for it.
+struct RowGrad {
+  float m = 0.f, mass_over_s = 0.f, scale = 0.f, shift = 0.f;
+};
+
+// The row's loss before its weight, and the gradient's factors. One thread's work.
+__device__ __forceinline__ float finish_loss(const Record& r, const RecordSums* part, const Soft& soft, RowGrad& g) {
+  RecordSums t = part[0];
+  for (uint32_t w = 1; w * 32 < r.k; ++w) t.merge(part[w]);
+  g = RowGrad{};
+  if (t.q == 0.0) return 0.f;                // no mass on record
+  if (soft.m == -INFINITY) return INFINITY;  // no finite logit
+  g.m = soft.m;
+  g.shift = t.shift;
   const double scale = r.renormalize ? 1.0 / t.q : 1.0;
-  g.q_scale = (float)scale;
+  g.scale = (float)scale;
   g.mass_over_s = (float)(t.q * scale / (double)soft.s);
   const double log_s = log((double)soft.s);
-  if (r.renormalize) return (float)((t.q_lp - t.q_d) * scale - (log(t.q) + (double)t.shift) + log_s);
-  return (float)(t.q_lp - t.q_d + t.q * log_s);
+  const double q_d = (t.q_x + t.q * ((double)t.at - (double)soft.m)) * (double)r.inv_t;
+  if (r.renormalize) return (float)((t.q_lp - q_d) * scale - (log(t.q) + (double)t.shift) + log_s);
+  return (float)(t.q_lp - q_d + t.q * log_s);
 }
 
-// Writes units [first, last) of one gradient row: dense part a * 2^((x - m) c), then the record's
-// corrections that fall among them.
+struct GradShared {
+  int ids[WS_TOP_MAX_K];
+  float qs[WS_TOP_MAX_K];
+};
+
+// One step's units of a gradient row: a 2^((x - m) c), or zeros.
 template <class T>
-__device__ __forceinline__ void write_grad(const Record& r, uint32_t row, const RowWalk<T>& walk, uint32_t first, uint32_t last,
-                                           T* grad, uint32_t vocab, float m, float shift, float a, float b, int* ids, float* qs) {
-  // a = g w Q / (t S), b = g w q_scale / t, q = exp(lp - shift); both 0: the row has no gradient and its logits are not read.
-  const bool none = a == 0.f && b == 0.f;
-  T* out = grad - walk.head;  // by aligned position
-  const bool same = (((uintptr_t)out) & 15u) == 0;
-  const uint64_t nm = pair(-m, -m), cc = pair(r.c, r.c), aa = pair(a, a);
-  Batch<T> next;
-  if (none) next = Batch<T>{};
-  else if (first < last) next.load(walk, first, last);
-  for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
-    const Batch<T> now = next;
-    if (!none && u0 + Batch<T>::kSpan < last) next.load(walk, u0 + Batch<T>::kSpan, last);
+__device__ __forceinline__ void write_step(const RowWalk<T>& walk, T* out, bool wide, uint32_t u0, uint32_t last, const Batch<T>& b,
+                                           float m, float c, float a) {
+  const uint64_t nm = pair(-m, -m), cc = pair(c, c), aa = pair(a, a);
 #pragma unroll
-    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
-      const uint32_t u = u0 + j * kRowThreads + threadIdx.x;
-      if (u >= last) continue;
-      float f[kUnit];
-      unpack<T>(now.raw[j], f);
-      if (!none) {
+  for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+    const uint32_t u = Batch<T>::unit(u0, j);
+    if (u >= last) continue;
+    float f[kUnit<T>];
+    unpack<T>(b.raw[j], f);
 #pragma unroll
-        for (uint32_t i = 0; i < kUnit; i += 2) {
-          const float2 e = unpair(mul2(add2(pair(f[i], f[i + 1]), nm), cc));
-          const float2 g = unpair(mul2(aa, pair(ex2(e.x), ex2(e.y))));
-          f[i] = g.x;
-          f[i + 1] = g.y;
-        }
-      }
-      if (same && walk.whole(u)) {
-        const Raw<T> w = pack<T>(f);
-        uint4* v = reinterpret_cast<uint4*>(out + (size_t)u * kUnit);
+    for (uint32_t i = 0; i < kUnit<T>; i += 2) {
+      const float2 e = unpair(mul2(add2(pair(f[i], f[i + 1]), nm), cc));
+      const float2 g = unpair(mul2(aa, pair(ex2(e.x), ex2(e.y))));
+      f[i] = g.x;
+      f[i + 1] = g.y;
+    }
+    if (wide && walk.whole(u)) {
+      reinterpret_cast<uint4*>(out)[u] = pack<T>(f);
+    } else {
 #pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) / 2; ++i) v[i] = w.v[i];
-      } else {
-#pragma unroll
-        for (uint32_t i = 0; i < kUnit; ++i) {
-          const uint32_t p = u * kUnit + i;
-          if (p >= walk.head && p < walk.end) out[p] = from_float<T>(f[i]);
-        }
+      for (uint32_t i = 0; i < kUnit<T>; ++i) {
+        const uint32_t p = u * kUnit<T> + i;
+        if (p >= walk.head && p < walk.end) out[p] = from_float<T>(f[i]);
       }
     }
   }
-  if (none) return;  // the same for the whole block
-  int id;
-  float lp;
-  record_entry(r, row, threadIdx.x, vocab, id, lp);
-  ids[threadIdx.x] = id;
-  qs[threadIdx.x] = id >= 0 ? expf(lp - shift) : 0.f;
-  __syncthreads();  // the dense part is written, too
-  const uint32_t p = (uint32_t)id + walk.head;
-  if (id >= 0 && p >= first * kUnit && p < last * kUnit) {
+}
+
+template <class T>
+__device__ __forceinline__ void write_zeros(const RowWalk<T>& walk, T* out, bool wide, uint32_t first, uint32_t last) {
+  for (uint32_t u = first + threadIdx.x; u < last; u += kRowThreads) {
+    if (wide && walk.whole(u)) {
+      reinterpret_cast<uint4*>(out)[u] = make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < kUnit<T>; ++i) {
+        const uint32_t p = u * kUnit<T> + i;
+        if (p >= walk.head && p < walk.end) out[p] = from_float<T>(0.f);
+      }
+    }
+  }
+}
+
+// The elements of units [first, last) that the record names, behind the dense part: each once, by the first entry that names it.
+template <class T>
+__device__ __forceinline__ void write_record(const Record& r, const Entry& e, const RowWalk<T>& walk, T* out, uint32_t first,
+                                             uint32_t last, const RowGrad& g, float a, float b, GradShared& s) {
+  s.ids[threadIdx.x] = e.id;
+  s.qs[threadIdx.x] = e.id >= 0 ? expf(e.lp - g.shift) : 0.f;
+  __syncthreads();  // the block's dense part is written, too
+  const uint32_t p = (uint32_t)e.id + walk.head;
+  if (e.id >= 0 && p >= first * kUnit<T> && p < last * kUnit<T>) {
     float q = 0.f;
     bool owner = true;
+#pragma unroll 4
     for (uint32_t j = 0; j < r.k; ++j) {
-      if (ids[j] == id) {
+      if (s.ids[j] == e.id) {
         owner = owner && j >= threadIdx.x;
-        q += qs[j];
+        q += s.qs[j];
       }
     }
-    if (owner) out[p] = from_float<T>(a * ex2((walk.at(p) - m) * r.c) - b * q);
+    if (owner) out[p] = from_float<T>(a * ex2((e.x - g.m) * r.c) - b * q);
   }
 }
 
 template <class T>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 4)
     distill_forward_kernel(RowSet x, Record r, float* __restrict__ loss, float* __restrict__ stats) {
-  __shared__ float2 soft_scratch[kRowWarps];
-  __shared__ float2 mine;
-  __shared__ double sums[kRowWarps];
-  const cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / blocks;
+  extern __shared__ __align__(16) uint8_t ring_memory[];
+  __shared__ float2 soft_scratch[kRowWarps], soft_slots[RowCluster::kMost];
+  __shared__ RecordSums part[kRowWarps];
+  const RowCluster cluster;
+  const uint32_t row = cluster.row();
   const float w = r.weights ? r.weights[row] : 1.f;
   float2* out = reinterpret_cast<float2*>(stats) + row;
   if (w == 0.f) {  // the same for the whole cluster
-    if (rank == 0 && threadIdx.x == 0) {
+    if (cluster.rank == 0 && threadIdx.x == 0) {
       loss[row] = 0.f;
       *out = make_float2(0.f, 0.f);
     }
     return;
   }
+  cluster.started();
   const T* src = row_ptr<T>(x, row);
   const RowWalk<T> walk(src, x.vocab);
   uint32_t first, last;
-  split_units(walk.units, rank, blocks, first, last);
-  const Soft soft = cluster_soft(row_soft(walk, first, last, r.c, soft_scratch), r.c, &mine);
-  if (rank == 0) {
-    const RecordSums t = record_sums<T>(r, row, src, x.vocab, soft.m, sums);
-    if (threadIdx.x == 0) {
-      RowGrad g;
-      loss[row] = w * finish_loss(r, t, soft, g);
-      *out = make_float2(g.m, g.mass_over_s);
-    }
+  split_units(walk.units, cluster.rank, cluster.blocks, first, last);
+  Ring<T, kDepth> ring(ring_memory, walk, first, last);
+  if (cluster.rank == 0) {  // while the first copies are on their way
+    Entry e;
+    e.load(r, row, src, x.vocab);
+    sum_record(r, e, part);
   }
-  if (blocks > 1) cluster.sync();  // `mine` is read until here
+  Soft soft = row_soft(ring, first, last, r.c, soft_scratch);
+  if (cluster.blocks > 1) {
+    cluster.ready();
+    tell_soft(cluster, soft, soft_slots);
+    cluster.told();
+    soft = told_soft(cluster, r.c, soft_slots);
+  }
+  if (cluster.rank == 0 && threadIdx.x == 0) {
+    RowGrad g;
+    loss[row] = w * finish_loss(r, part, soft, g);
+    *out = make_float2(g.m, g.mass_over_s);
+  }
 }
 
 template <class T>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 4)
     distill_backward_kernel(RowSet x, Record r, const float* __restrict__ stats, const float* __restrict__ grad_loss,
                             int64_t grad_outer, int64_t grad_inner, RowSet dx) {
-  __shared__ int ids[kRowThreads];
-  __shared__ float qs[kRowThreads];
-  __shared__ double sums[kRowWarps];
-  const cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t pieces = cluster.num_blocks(), piece = cluster.block_rank(), row = blockIdx.x / pieces;
+  extern __shared__ __align__(16) uint8_t ring_memory[];
+  __shared__ GradShared s;
+  __shared__ RecordSums part[kRowWarps];
+  const RowCluster cluster;  // its blocks have nothing to tell each other here
+  const uint32_t row = cluster.row();
   const float w = r.weights ? r.weights[row] : 1.f;
   const float2 st = reinterpret_cast<const float2*>(stats)[row];
   const uint32_t o = row / x.inner, in = row - o * x.inner;
-  float a = 0.f, b = 0.f, shift = 0.f;
-  if (w != 0.f && st.y != 0.f) {
-    const float g = grad_loss[(int64_t)o * grad_outer + (int64_t)in * grad_inner] * w * r.inv_t;
-    float scale = 1.f;
-    if (r.renormalize) {
-      int id;
-      float lp;
-      record_entry(r, row, threadIdx.x, x.vocab, id, lp);
-      shift = record_shift(r, id, lp, reinterpret_cast<float*>(sums));
-      scale = (float)(1.0 / block_sum(id >= 0 ? exp((double)lp - (double)shift) : 0.0, sums));
-    }
-    a = g * st.y;
-    b = g * scale;
-  }
-  const RowWalk<T> walk(row_ptr<T>(x, row), x.vocab);
+  const float g = grad_loss[(int64_t)o * grad_outer + (int64_t)in * grad_inner] * w * r.inv_t;
+  const T* src = row_ptr<T>(x, row);
+  const RowWalk<T> walk(src, x.vocab);
   uint32_t first, last;
-  split_units(walk.units, piece, pieces, first, last);
-  write_grad<T>(r, row, walk, first, last, row_ptr<T>(dx, row), x.vocab, st.x, shift, a, b, ids, qs);
+  split_units(walk.units, cluster.rank, cluster.blocks, first, last);
+  T* out = row_ptr<T>(dx, row) - walk.head;  // by aligned position
+  const bool wide = ((uintptr_t)out & 15u) == 0;
+  if (w == 0.f || g == 0.f || st.y == 0.f) {
+    write_zeros(walk, out, wide, first, last);
+    return;
+  }
+  Ring<T, kDepth> ring(ring_memory, walk, first, last);
+  Entry e;
+  e.load(r, row, src, x.vocab);
+  if (r.renormalize) sum_record(r, e, part);
+  const float a = g * st.y;
+  for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
+    Batch<T> b;
+    ring.read(b);
+    write_step(walk, out, wide, u0, last, b, st.x, r.c, a);
+    ring.advance();
+  }
+  RowGrad f{st.x, st.y, 1.f, 0.f};
+  if (r.renormalize) {
+    __syncthreads();
+    RecordSums t = part[0];
+    for (uint32_t i = 1; i * 32 < r.k; ++i) t.merge(part[i]);
+    f.scale = (float)(1.0 / t.q);
+    f.shift = t.shift;
+  }
+  write_record(r, e, walk, out, first, last, f, a, g * f.scale, s);
 }
 
 template <class T>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 3)
     distill_step_kernel(RowSet x, Record r, float* __restrict__ loss, RowSet dx) {
-  __shared__ float2 soft_scratch[kRowWarps];
-  __shared__ float2 mine;
-  __shared__ double sums[kRowWarps];
-  __shared__ int ids[kRowThreads];
-  __shared__ float qs[kRowThreads];
-  const cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / blocks;
+  extern __shared__ __align__(16) uint8_t ring_memory[];
+  __shared__ float2 soft_scratch[kRowWarps], soft_slots[RowCluster::kMost];
+  __shared__ RecordSums part[kRowWarps];
+  __shared__ GradShared s;
+  __shared__ RowGrad shared_grad;
+  const RowCluster cluster;
+  const uint32_t row = cluster.row();
   const float w = r.weights ? r.weights[row] : 1.f;
   const T* src = row_ptr<T>(x, row);
   const RowWalk<T> walk(src, x.vocab);
   uint32_t first, last;
-  split_units(walk.units, rank, blocks, first, last);
-  float m = 0.f, shift = 0.f, a = 0.f, b = 0.f, l = 0.f;
-  if (w != 0.f) {  // the same for the whole cluster
-    const Soft soft = cluster_soft(row_soft(walk, first, last, r.c, soft_scratch), r.c, &mine);
-    const RecordSums t = record_sums<T>(r, row, src, x.vocab, soft.m, sums);
-    RowGrad g;
-    l = w * finish_loss(r, t, soft, g);
-    m = g.m;
-    shift = t.shift;
-    a = w * r.inv_t * g.mass_over_s;
-    b = w * r.inv_t * g.q_scale;
+  split_units(walk.units, cluster.rank, cluster.blocks, first, last);
+  T* out = row_ptr<T>(dx, row) - walk.head;
+  const bool wide = ((uintptr_t)out & 15u) == 0;
+  if (w == 0.f) {  // the same for the whole cluster
+    if (cluster.rank == 0 && threadIdx.x == 0) loss[row] = 0.f;
+    write_zeros(walk, out, wide, first, last);
+    return;
   }
-  if (rank == 0 && threadIdx.x == 0) loss[row] = l;
-  write_grad<T>(r, row, walk, first, last, row_ptr<T>(dx, row), x.vocab, m, shift, a, b, ids, qs);
-  if (blocks > 1) cluster.sync();  // `mine` is read until here
+  cluster.started();
+  Ring<T, kStepDepth> ring(ring_memory, walk, first, last);
+  Entry e;
+  e.load(r, row, src, x.vocab);
+  sum_record(r, e, part);
+  Soft soft = row_soft(ring, first, last, r.c, soft_scratch);
+  if (cluster.blocks > 1) {
+    cluster.ready();
+    tell_soft(cluster, soft, soft_slots);
+    cluster.told();
+    soft = told_soft(cluster, r.c, soft_slots);
+  }
+  if (threadIdx.x == 0) {
+    RowGrad g;
+    const float l = w * finish_loss(r, part, soft, g);
+    if (cluster.rank == 0) loss[row] = l;
+    shared_grad = g;
+  }
+  __syncthreads();
+  const RowGrad g = shared_grad;
+  const float a = w * r.inv_t * g.mass_over_s, b = w * r.inv_t * g.scale;
+  if (g.mass_over_s == 0.f) {
+    write_zeros(walk, out, wide, first, last);
+    return;
+  }
+  // The second pass, from shared memory where the block's share is still there.
+  if (last - first <= kStepDepth * Batch<T>::kSpan) {
+    uint32_t slot = 0;
+    for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan, ++slot) {
+      Batch<T> t;
+      ring.again(slot, t);
+      write_step(walk, out, wide, u0, last, t, g.m, r.c, a);
+    }
+  } else {
+    Ring<T, kStepDepth> second(ring_memory, walk, first, last);
+    for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
+      Batch<T> t;
+      second.read(t);
+      write_step(walk, out, wide, u0, last, t, g.m, r.c, a);
+      second.advance();
+    }
+  }
+  write_record(r, e, walk, out, first, last, g, a, b, s);
 }
 
 int fail(int code, const std::string& msg) {
@@ -333,7 +431,7 @@ extern "C" int ws_distill_forward(const ws_rows* logits, const ws_teacher* teach
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(distill_forward_kernel<T>, x.rows, blocks_a_row(x.rows, x.set.vocab / kUnit), stream, x.set, r, loss, stats);
+        return launch_rows<distill_forward_kernel<T>>(x.rows, blocks_a_row(x), kDepth * kStepBytes, device, stream, x.set, r, loss, stats);
       });
     return done(e, "distill forward");
   });
@@ -353,13 +451,13 @@ extern "C" int ws_distill_backward(const ws_rows* logits, const ws_teacher* teac
     if (x.rows == 0) return (int)WS_OK;
     if (!stats || !grad_loss) return fail(WS_ERR_INVALID, "null pointer");
     if ((uintptr_t)stats % 8) return fail(WS_ERR_INVALID, "stats must be 8-byte aligned");
-    const uint32_t pieces = blocks_a_row(x.rows, x.set.vocab / kUnit);
+    const uint32_t pieces = blocks_a_row(x);
     DeviceGuard guard(device);
     cudaError_t e = guard.error();
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(distill_backward_kernel<T>, x.rows, pieces, stream, x.set, r, stats, grad_loss, grad_outer, grad_inner, dx.set);
+        return launch_rows<distill_backward_kernel<T>>(x.rows, pieces, kDepth * kStepBytes, device, stream, x.set, r, stats, grad_loss, grad_outer, grad_inner, dx.set);
       });
     return done(e, "distill backward");
   });
@@ -382,7 +480,7 @@ extern "C" int ws_distill_step(const ws_rows* logits, const ws_teacher* teacher,
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(distill_step_kernel<T>, x.rows, blocks_a_row(x.rows, x.set.vocab / kUnit), stream, x.set, r, loss, dx.set);
+        return launch_rows<distill_step_kernel<T>>(x.rows, blocks_a_row(x), kStepDepth * kStepBytes, device, stream, x.set, r, loss, dx.set);
       });
     return done(e, "distill step");
   });

@@ -18,26 +18,35 @@ namespace cg = cooperative_groups;
 // larger one comes first in the record.
 //
 // What a logit costs is one comparison of its unit's maximum with a threshold, below which nothing can be in
-// the record. The threshold comes from maxima that are at hand anyway: every thread keeps the maximum of each
-// of its kUnits places in a step over all steps, kRowThreads * kUnits logits of different
-// ids, the k-th largest of which is a lower bound of the k-th largest logit, and a close one. It is
-// found by bisection over the upper 16 bits of the order keys after steps 1, 2, 4, 8, ...
-// and at the end, when the list holds few more than k candidates.
+// the record. The threshold comes from maxima that are at hand anyway: every thread keeps the maximum of what it
+// has seen (for records of more than kFewMaxima, one for each of its kUnits places in a step), which is
+// kRowThreads or more logits of different ids, and the k-th largest of those is a lower bound of the k-th
+// largest logit, and a close one. It is found by bisection over the upper 16 bits of the order keys after steps
+// 1, 4, 16, 64 and at the end; meanwhile a step adds about k candidates divided by the steps before the last
+// threshold.
 //
 // The list has room for k candidates and all of a step's that one unit of each thread
 // gives. A step that would overflow it (ascending or equal logits) is taken again unit
 // by unit, dropping all but the k largest before each: slow, and right for any row.
-constexpr uint32_t kCandidates = WS_TOP_MAX_K + kRowThreads * kUnit;
+constexpr uint32_t kTopDepth = 2;    // steps in flight
+constexpr uint32_t kFewMaxima = 64;
+constexpr uint32_t kCandidates = WS_TOP_MAX_K + kRowThreads * 8;
 constexpr uint32_t kSorted = 512;  // candidates that are put in order by counting
 
 struct TopShared {
   uint64_t list[kCandidates];
-  uint64_t sorted[WS_TOP_MAX_K];  // the block's k largest in order, for the other blocks of the cluster
+  uint64_t sorted[WS_TOP_MAX_K];  // the block's k largest in order
   uint32_t count, sorted_count;
   uint32_t sums[kRowWarps];
   uint2 votes[2][kRowWarps];
   float2 soft[kRowWarps];
-  float2 soft_mine;
+};
+
+// What the blocks of a cluster tell each other of their shares of a row.
+struct TopTold {
+  uint64_t lists[RowCluster::kMost][WS_TOP_MAX_K];
+  uint32_t counts[RowCluster::kMost];
+  float2 soft[RowCluster::kMost];
 };
 
 __device__ __forceinline__ uint64_t candidate(float x, uint32_t id) { return ((uint64_t)order_key(x) << 32) | (0xFFFFFFFFu - id); }
@@ -71,14 +80,14 @@ __device__ __noinline__ uint64_t keep_largest(TopShared& s, uint32_t n, uint32_t
 
 // A logit that at least k of the block's maxima reach, as large as 16 bits of its order key
 // tell; the lowest finite number where fewer than k are above -inf. Two bits a round: the
-// counts of three trials by one shuffle-free reduction in the warp, and one barrier.
+// counts of three trials by one reduction in the warp and one barrier.
 template <uint32_t N>
 __device__ __forceinline__ float kth_of_maxima(TopShared& s, const float (&top)[N], uint32_t k) {
   uint32_t key[N];
 #pragma unroll
   for (uint32_t j = 0; j < N; ++j) key[j] = order_key(top[j]) >> 16;
   uint32_t edge = 0;
-#pragma unroll
+#pragma unroll 1
   for (int bit = 14; bit >= 0; bit -= 2) {
     uint32_t low = 0, high = 0;  // counts of trials 1 and 2, and of trial 3
 #pragma unroll
@@ -104,44 +113,82 @@ __device__ __forceinline__ float kth_of_maxima(TopShared& s, const float (&top)[
   return edge <= kNone ? -FLT_MAX : key_value(edge << 16);
 }
 
-// The statistics and the k largest logits of units [first, last) of a row: s.sorted_count (at most k) candidates in s.sorted, in
-// order. Every thread gets the statistics.
-template <class T>
-__device__ __forceinline__ Soft row_top(const RowWalk<T>& walk, uint32_t first, uint32_t last, float c, uint32_t k, TopShared& s) {
-  using B = Batch<T>;
-  if (threadIdx.x == 0) s.count = 0;
-  Soft soft;
-  float most[B::kUnits];
+template <uint32_t N>
+__device__ __forceinline__ float kth_threshold(TopShared& s, const float (&most)[N], uint32_t k) {
+  if (k > kFewMaxima) return kth_of_maxima(s, most, k);
+  float one[1] = {most[0]};
 #pragma unroll
-  for (uint32_t j = 0; j < B::kUnits; ++j) most[j] = -INFINITY;
-  float edge = -FLT_MAX;  // logits below it are of no use; nor are -inf and NaN
-  B next;
-  if (first < last) next.load(walk, first, last);
+  for (uint32_t j = 1; j < N; ++j) one[0] = fmaxf(one[0], most[j]);
+  return kth_of_maxima(s, one, k);
+}
+
+// The step that begins at unit u0 again, from the `before` candidates there were, unit by unit; returns the new threshold.
+template <class T>
+__device__ __noinline__ float top_overflow(TopShared& s, Batch<T> now, uint32_t u0, uint32_t before, uint32_t k, uint32_t head,
+                                           float edge) {
   __syncthreads();
-  uint32_t step = 1;
-  for (uint32_t u0 = first; u0 < last; u0 += B::kSpan, ++step) {
-    const B now = next;
-    if (u0 + B::kSpan < last) next.load(walk, u0 + B::kSpan, last);
-    float top[B::kUnits], all = -INFINITY;
+  if (threadIdx.x == 0) s.count = before;
+  __syncthreads();
+  uint64_t least = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+    if (s.count > k) least = keep_largest(s, s.count, k);
+    __syncthreads();
+    float f[kUnit<T>];
+    unpack<T>(now.raw[j], f);
+    const uint32_t id = Batch<T>::unit(u0, j) * kUnit<T> - head;
+#pragma unroll
+    for (uint32_t i = 0; i < kUnit<T>; ++i) {
+      if (f[i] >= edge) {
+        const uint64_t v = candidate(f[i], id + i);
+        if (v > least) s.list[atomicAdd(&s.count, 1u)] = v;
+      }
+    }
+    __syncthreads();
+  }
+  if (s.count > k) least = keep_largest(s, s.count, k);
+  __syncthreads();
+  return fmaxf(edge, least ? candidate_value(least) : -FLT_MAX);
+}
+
+// The k largest logits of what the block has read so far.
+template <class T>
+struct TopCollector {
+  using B = Batch<T>;
+  TopShared& s;
+  uint32_t k, head, step = 1;
+  float edge = -FLT_MAX;  // logits below it are of no use; nor are -inf and NaN
+  float most[B::kUnits];
+
+  __device__ __forceinline__ TopCollector(TopShared& shared, uint32_t k_, uint32_t head_) : s(shared), k(k_), head(head_) {
+    if (threadIdx.x == 0) s.count = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < B::kUnits; ++j) most[j] = -INFINITY;
+    __syncthreads();
+  }
+
+  // The step that begins at unit u0; top: the maxima of the thread's units in it.
+  __device__ __forceinline__ void add(const B& now, const float (&top)[B::kUnits], uint32_t u0) {
+    float all = top[0];
 #pragma unroll
     for (uint32_t j = 0; j < B::kUnits; ++j) {
-      top[j] = unit_max<T>(now.raw[j]);
       most[j] = fmaxf(most[j], top[j]);
       all = fmaxf(all, top[j]);
     }
-    soft.add(now, all, c);
-    if ((step & (step - 1)) == 0) edge = fmaxf(edge, kth_of_maxima(s, most, k));
+    // Steps 1, 4, 16, 64, ...: powers of 4.
+    if ((step & (step - 1)) == 0 && (step & 0x55555555u)) edge = fmaxf(edge, kth_threshold(s, most, k));
+    ++step;
     const uint32_t before = s.count;
     __syncthreads();  // everyone has it
     if (all >= edge) {
 #pragma unroll
       for (uint32_t j = 0; j < B::kUnits; ++j) {
         if (top[j] >= edge) {
-          float f[kUnit];
+          float f[kUnit<T>];
           unpack<T>(now.raw[j], f);
-          const uint32_t id = (u0 + j * kRowThreads + threadIdx.x) * kUnit - walk.head;
+          const uint32_t id = B::unit(u0, j) * kUnit<T> - head;
 #pragma unroll
-          for (uint32_t i = 0; i < kUnit; ++i) {
+          for (uint32_t i = 0; i < kUnit<T>; ++i) {
             if (f[i] >= edge) {
               const uint32_t at = atomicAdd(&s.count, 1u);
               if (at < kCandidates) s.list[at] = candidate(f[i], id + i);
@@ -151,76 +198,49 @@ __device__ __forceinline__ Soft row_top(const RowWalk<T>& walk, uint32_t first, 
       }
     }
     __syncthreads();
-    if (s.count > kCandidates) {
-      __syncthreads();
-      if (threadIdx.x == 0) s.count = before;
-      __syncthreads();
-      uint64_t least = 0;
-      for (uint32_t j = 0; j < B::kUnits; ++j) {
-        if (s.count > k) least = keep_largest(s, s.count, k);
-        __syncthreads();
-        Raw<T> raw = now.raw[0];
+    if (s.count > kCandidates) edge = top_overflow<T>(s, now, u0, before, k, head, edge);
+  }
+
+  // s.sorted_count (at most k) candidates in s.sorted, in order; visible behind the next barrier.
+  __device__ __forceinline__ void finish() {
+    edge = fmaxf(edge, kth_threshold(s, most, k));
+    constexpr uint32_t kMine = (kCandidates + kRowThreads - 1) / kRowThreads;
+    const uint32_t found = s.count;
+    uint64_t mine[kMine];
 #pragma unroll
-        for (uint32_t q = 1; q < B::kUnits; ++q)
-          if (q == j) raw = now.raw[q];
-        float f[kUnit];
-        unpack<T>(raw, f);
-        const uint32_t id = (u0 + j * kRowThreads + threadIdx.x) * kUnit - walk.head;
+    for (uint32_t i = 0; i < kMine; ++i) {
+      const uint32_t at = i * kRowThreads + threadIdx.x;
+      mine[i] = at < found ? s.list[at] : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
 #pragma unroll
-        for (uint32_t i = 0; i < kUnit; ++i) {
-          if (f[i] >= edge) {
-            const uint64_t v = candidate(f[i], id + i);
-            if (v > least) s.list[atomicAdd(&s.count, 1u)] = v;
-          }
-        }
-        __syncthreads();
-      }
-      if (s.count > k) least = keep_largest(s, s.count, k);
-      edge = fmaxf(edge, least ? candidate_value(least) : -FLT_MAX);
-      __syncthreads();
+    for (uint32_t i = 0; i < kMine; ++i)
+      if (mine[i] && candidate_value(mine[i]) >= edge) s.list[atomicAdd(&s.count, 1u)] = mine[i];
+    __syncthreads();
+    if (s.count > kSorted) keep_largest(s, s.count, k);  // k <= WS_TOP_MAX_K <= kSorted remain
+    const uint32_t n = s.count;
+    if (threadIdx.x == 0) s.sorted_count = min(n, k);
+    for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) {
+      const uint64_t v = s.list[i];
+      uint32_t place = 0;
+#pragma unroll 4
+      for (uint32_t q = 0; q < n; ++q) place += s.list[q] > v;
+      if (place < k) s.sorted[place] = v;
     }
   }
-  // Of the candidates those that reach the last threshold, in order. A thread holds at most kMine of them.
-  edge = fmaxf(edge, kth_of_maxima(s, most, k));
-  constexpr uint32_t kMine = (kCandidates + kRowThreads - 1) / kRowThreads;
-  uint64_t mine[kMine];
-  const uint32_t found = s.count;
-#pragma unroll
-  for (uint32_t i = 0; i < kMine; ++i) {
-    const uint32_t at = i * kRowThreads + threadIdx.x;
-    mine[i] = at < found ? s.list[at] : 0;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) s.count = 0;
-  __syncthreads();
-#pragma unroll
-  for (uint32_t i = 0; i < kMine; ++i)
-    if (mine[i] && candidate_value(mine[i]) >= edge) s.list[atomicAdd(&s.count, 1u)] = mine[i];
-  __syncthreads();
-  if (s.count > kSorted) keep_largest(s, s.count, k);  // k <= WS_TOP_MAX_K <= kSorted remain
-  const uint32_t n = s.count;
-  if (threadIdx.x == 0) s.sorted_count = min(n, k);
-  for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) {
-    const uint64_t v = s.list[i];
-    uint32_t place = 0;
-#pragma unroll 4
-    for (uint32_t q = 0; q < n; ++q) place += s.list[q] > v;
-    if (place < k) s.sorted[place] = v;
-  }
-  return block_soft(soft, c, s.soft);  // with a barrier behind s.sorted
-}
+};
 
-// The cluster's record: place of this block's i-th candidate, which is i and how many of the other blocks' are larger.
-__device__ __forceinline__ uint32_t cluster_place(TopShared& s, uint32_t i, uint64_t v) {
-  cg::cluster_group cluster = cg::this_cluster();
+// The place of this block's i-th candidate in the cluster's record: i and how many of the other blocks' are larger.
+__device__ __forceinline__ uint32_t cluster_place(const RowCluster& cluster, const TopTold& told, uint32_t i, uint64_t v) {
   uint32_t place = i;
-  for (uint32_t b = 0; b < cluster.num_blocks(); ++b) {
-    if (b == cluster.block_rank()) continue;
-    const TopShared* o = cluster.map_shared_rank(&s, b);
-    uint32_t lo = 0, hi = o->sorted_count;
+  for (uint32_t b = 0; b < cluster.blocks; ++b) {
+    if (b == cluster.rank) continue;
+    uint32_t lo = 0, hi = told.counts[b];
     while (lo < hi) {
       const uint32_t mid = (lo + hi) / 2;
-      if (o->sorted[mid] > v) lo = mid + 1;
+      if (told.lists[b][mid] > v) lo = mid + 1;
       else hi = mid;
     }
     place += lo;
@@ -228,35 +248,73 @@ __device__ __forceinline__ uint32_t cluster_place(TopShared& s, uint32_t i, uint
   return place;
 }
 
+// The block's sorted candidates into every block's `told`; between ready() and told().
+__device__ __forceinline__ void tell_top(const RowCluster& cluster, const TopShared& s, TopTold* told) {
+  const uint32_t n = s.sorted_count;
+  for (uint32_t b = 0; b < cluster.blocks; ++b) {
+    TopTold* to = cluster.of(told, b);
+    if (threadIdx.x < n) to->lists[cluster.rank][threadIdx.x] = s.sorted[threadIdx.x];
+    if (threadIdx.x == 0) to->counts[cluster.rank] = n;
+  }
+}
+
 template <class T>
 __global__ void __launch_bounds__(kRowThreads, 3)
     top_kernel(RowSet x, uint32_t k, float c, float inv_t, int64_t* __restrict__ ids, float* __restrict__ logprobs) {
+  // The ring, and behind it, where the row has several blocks, what they tell each other.
+  extern __shared__ __align__(16) uint8_t memory[];
   __shared__ TopShared s;
-  cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / blocks;
+  const RowCluster cluster;
+  cluster.started();
+  const uint32_t row = cluster.row();
   const RowWalk<T> walk(row_ptr<T>(x, row), x.vocab);
   uint32_t first, last;
-  split_units(walk.units, rank, blocks, first, last);
-  const Soft soft = cluster_soft(row_top(walk, first, last, c, k, s), c, &s.soft_mine);
+  split_units(walk.units, cluster.rank, cluster.blocks, first, last);
+  Ring<T, kTopDepth> ring(memory, walk, first, last);
+  TopCollector<T> top(s, k, walk.head);
+  Soft soft;
+  for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
+    Batch<T> b;
+    ring.read(b);
+    float most[Batch<T>::kUnits], all = -INFINITY;
+#pragma unroll
+    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+      most[j] = unit_max<T>(b.raw[j]);
+      all = fmaxf(all, most[j]);
+    }
+    soft.add(b, all, c);
+    top.add(b, most, u0);
+    ring.advance();
+  }
+  top.finish();
+  soft = block_soft(soft, c, s.soft);  // a barrier behind s.sorted, too
+  uint32_t n = s.sorted_count;
+  TopTold* told = reinterpret_cast<TopTold*>(memory + kTopDepth * kStepBytes);
+  if (cluster.blocks > 1) {
+    cluster.ready();
+    tell_soft(cluster, soft, told->soft);
+    tell_top(cluster, s, told);
+    cluster.told();
+    soft = told_soft(cluster, c, told->soft);
+    n = 0;
+    for (uint32_t b = 0; b < cluster.blocks; ++b) n += told->counts[b];
+  }
   const double log_s = log((double)soft.s);
   const size_t out = (size_t)row * k;
   if (threadIdx.x < s.sorted_count) {
     const uint64_t v = s.sorted[threadIdx.x];
-    const uint32_t place = blocks > 1 ? cluster_place(s, threadIdx.x, v) : threadIdx.x;
+    const uint32_t place = cluster.blocks > 1 ? cluster_place(cluster, *told, threadIdx.x, v) : threadIdx.x;
     if (place < k) {
       ids[out + place] = (int64_t)(0xFFFFFFFFu - (uint32_t)v);
       logprobs[out + place] = (float)(((double)candidate_value(v) - (double)soft.m) * (double)inv_t - log_s);
     }
   }
-  if (rank == 0) {
-    uint32_t n = 0;
-    for (uint32_t b = 0; b < blocks; ++b) n += cluster.map_shared_rank(&s, b)->sorted_count;
+  if (cluster.rank == 0) {
     for (uint32_t i = n + threadIdx.x; i < k; i += kRowThreads) {
       ids[out + i] = -1;
       logprobs[out + i] = isnan(soft.s) ? NAN : -INFINITY;
     }
   }
-  if (blocks > 1) cluster.sync();  // the blocks' shared memory is read until here
 }
 
 // ------------------------------------------------------------ sampling
@@ -266,40 +324,83 @@ __global__ void __launch_bounds__(kRowThreads, 3)
 // with the lowest ids). Weights are 2^42 exp((x - m) / t) rounded to integers: 2^20 of
 // them fit 64 bits, sums are exact whatever their order, and what rounding and the 64-bit
 // exponential leave off is below 2^-42 of the largest weight a token.
+//
+// One pass over the row gives (m, s) of every chunk (a warp's share of a step), in fp32, and, where tokens
+// are to be dropped, the largest logits as for a record. Most rows are decided by these:
+//   - all tokens kept: u times the total falls into a chunk, and within the chunk
+//     between two tokens, whose weights are computed as integers;
+//   - else, if the tokens kept are all among the largest ones at hand, these
+//     alone are weighed, as integers.
+// The total from fp32 sums is off by at most kSumError, relative (the exponential by 2^-22; its exponent by three
+// roundings, on exponents of at most 40 as far as they matter, 5e-6; 22 additions in a chain, 1.3e-6). Where
+// a border lies closer than that allows, and where more tokens are kept than are at hand, the row is
+// decided by exact_token, which weighs every token as an integer.
 constexpr uint32_t kBins = 1024;
-constexpr uint32_t kChunkUnits = 128;  // a warp's piece of the row when tokens are counted in id order
-constexpr uint32_t kChunk = kChunkUnits * kUnit;
-constexpr uint32_t kChunks = WS_MAX_VOCAB / kChunk + 1;
+constexpr uint32_t kChunkUnits = Batch<float>::kWarpSpan;  // of any type
+template <class T>
+constexpr uint32_t kChunk = kChunkUnits * kUnit<T>;
+constexpr uint32_t kChunks = WS_MAX_VOCAB / kChunk<float> + 1;
 constexpr double kWeightOne = 4398046511104.0;  // 2^42
+constexpr double kSumError = 1.0 / 131072;
+
+struct Bins {
+  uint32_t count[kBins];
+  unsigned long long mass[kBins];
+};
+struct ChunkSums {
+  unsigned long long mass[kChunks];
+  uint32_t ties[kChunks];
+};
+static_assert(sizeof(Bins) <= kTopDepth * kStepBytes && sizeof(ChunkSums) <= kTopDepth * kStepBytes, "they take the ring's place");
 
 struct SampleShared {
-  union {
-    struct {
-      uint32_t count[kBins];
-      unsigned long long mass[kBins];
-    } bins;
-    struct {
-      unsigned long long mass[kChunks];
-      uint32_t ties[kChunks];
-    } chunks;
-  };
+  TopShared top;
   struct {
     unsigned long long mass;
     uint32_t ties;
   } mine;  // for the other blocks of the cluster
-  unsigned long long sum_scratch[kRowWarps];
-  float2 soft_scratch[kRowWarps];
-  float2 soft_mine;
+  unsigned long long scan[kRowWarps];
+  double sums[kRowWarps];
+  unsigned long long weight[WS_TOP_MAX_K];
+  uint64_t merged[WS_TOP_MAX_K];  // the row's largest, in order, where it has several blocks
+  double chunk_before;
+  uint32_t chunk;
   uint32_t key_lo, key_hi;
-  uint32_t found_bin;
-  unsigned long long found_before, found_mass;
-  uint32_t found_count;
+  uint32_t found_bin, found_count;
+  unsigned long long found_before;
+  uint64_t token;  // token and the order key of its logit, in the lower half
 };
 
 __device__ __forceinline__ int64_t top_k_of(const ws_sampling& p, uint32_t row) {
   if (!p.top_k_each) return p.top_k;
   return p.top_k_is_int64 ? ((const int64_t*)p.top_k_each)[row] : (int64_t)((const int32_t*)p.top_k_each)[row];
 }
+
+// A row's settings; what is left of a temperature of 0 and of a top_p of 0 is top_k = 1.
+struct SampleSettings {
+  float t, top_p, min_p;
+  int64_t top_k;
+  double u;
+
+  __device__ __forceinline__ SampleSettings(const ws_sampling& p, const float* uniform, uint32_t row) {
+    t = p.temperature_each ? p.temperature_each[row] : p.temperature;
+    top_p = p.top_p_each ? p.top_p_each[row] : p.top_p;
+    min_p = fminf(p.min_p_each ? p.min_p_each[row] : p.min_p, 1.f);
+    top_k = top_k_of(p, row);
+    u = (double)uniform[row];
+    if (!(t > 0.f)) {
+      t = 1.f;
+      top_k = 1;
+    }
+    if (!(top_p > 0.f)) top_k = 1;
+  }
+  // A uniform number of 0 takes the first token of any weight, below 2^-43, too.
+  __device__ __forceinline__ bool first() const { return !(u > 0.0); }
+  // The cumulative weight that the token reaches first.
+  __device__ __forceinline__ unsigned long long need(unsigned long long total) const {
+    return first() ? 1 : min((unsigned long long)fmin(u * (double)total, 9e18) + 1, total);
+  }
+};
 
 // A row under its temperature; one block's part of it, in units [first, last).
 template <class T>
@@ -313,24 +414,69 @@ struct SampleRow {
   __device__ __forceinline__ unsigned long long fixed(float v) const {
     return v == m ? (unsigned long long)kWeightOne : __double2ull_rn(weight(v) * kWeightOne);
   }
-  // visit(logit, position) for every logit of the block's part above -inf.
+  // As it counts when the token is drawn.
+  __device__ __forceinline__ unsigned long long kept(float v, const SampleSettings& p) const {
+    const double w = weight(v);
+    if (p.min_p > 0.f && !(w >= (double)p.min_p)) return 0;
+    const unsigned long long f = __double2ull_rn(w * kWeightOne);
+    return p.first() && f == 0 && w > 0.0 ? 1 : f;
+  }
+  // visit(logit) for every logit of the block's part above -inf.
   template <class F>
   __device__ __forceinline__ void each(F&& visit) const {
     for (uint32_t u = first + threadIdx.x; u < last; u += kRowThreads) {
-      float f[kUnit];
+      float f[kUnit<T>];
       walk.load(u, f);
 #pragma unroll
-      for (uint32_t i = 0; i < kUnit; ++i)
-        if (f[i] > -INFINITY) visit(f[i], u * kUnit + i);
+      for (uint32_t i = 0; i < kUnit<T>; ++i)
+        if (f[i] > -INFINITY) visit(f[i]);
     }
   }
 };
 
+// Which tokens are kept: those with a logit above `edge`, and the first `ties` of those equal to it.
+struct Kept {
+  float edge = -INFINITY;
+  uint32_t ties = 0;
+};
+
+// The token of a chunk at which hit(weight before it, weight up to it), both counted from the chunk's begin, holds: into s.token.
+// `tied`: tokens equal to the edge before the chunk. The whole block calls it, and a barrier has to follow.
+template <class T, class H>
+__device__ __forceinline__ void find_in_chunk(SampleShared& s, const SampleRow<T>& row, const SampleSettings& p, uint32_t chunk,
+                                              const Kept& kept, uint32_t tied, H&& hit) {
+  constexpr uint32_t kMine = kChunk<T> / kRowThreads;
+  const uint32_t p0 = chunk * kChunk<T> + threadIdx.x * kMine;
+  const bool edged = kept.edge > -INFINITY;
+  float v[kMine];
+  uint32_t equal = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kMine; ++i) {
+    v[i] = p0 + i >= row.walk.head && p0 + i < row.walk.end ? row.walk.at(p0 + i) : -INFINITY;
+    equal += edged && v[i] == kept.edge;
+  }
+  uint32_t nth = tied, ties_all;
+  if (edged) nth += block_scan(equal, s.top.sums, &ties_all);
+  unsigned long long w[kMine], sum = 0, all;
+#pragma unroll
+  for (uint32_t i = 0; i < kMine; ++i) {
+    const bool tie = edged && v[i] == kept.edge;
+    w[i] = v[i] > kept.edge || (tie && nth < kept.ties) ? row.kept(v[i], p) : 0;
+    nth += tie;
+    sum += w[i];
+  }
+  unsigned long long before = block_scan(sum, s.scan, &all);
+#pragma unroll
+  for (uint32_t i = 0; i < kMine; ++i) {
+    if (w[i] && hit(before, before + w[i])) s.token = ((uint64_t)(p0 + i - row.walk.head) << 32) | order_key(v[i]);
+    before += w[i];
+  }
+}
+
 // Sum over the cluster; every thread of it gets it.
-template <class T>
-__device__ unsigned long long cluster_sum(unsigned long long v, SampleShared& s, const SampleRow<T>&) {
+__device__ __forceinline__ unsigned long long cluster_sum(unsigned long long v, SampleShared& s) {
   cg::cluster_group cluster = cg::this_cluster();
-  v = block_sum(v, s.sum_scratch);
+  v = block_sum(v, s.scan);
   if (threadIdx.x == 0) s.mine.mass = v;
   cluster.sync();
   unsigned long long t = 0;
@@ -343,16 +489,16 @@ __device__ unsigned long long cluster_sum(unsigned long long v, SampleShared& s,
 // `weigh`, their weight. Finds the lowest digit at which the running total (of counts, or of weights where
 // `weigh`) reaches `target`: s.found_*. The last bin, which may take most of a row, is counted in registers.
 template <class T, class D>
-__device__ void find_bin(SampleShared& s, const SampleRow<T>& row, bool weigh, unsigned long long target, D&& digit) {
+__device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, bool weigh, unsigned long long target, D&& digit) {
   cg::cluster_group cluster = cg::this_cluster();
   for (uint32_t i = threadIdx.x; i < kBins; i += kRowThreads) {
-    s.bins.count[i] = 0;
-    s.bins.mass[i] = 0;
+    bins.count[i] = 0;
+    bins.mass[i] = 0;
   }
   __syncthreads();
   uint32_t tail_count = 0;
   unsigned long long tail_mass = 0;
-  row.each([&](float v, uint32_t) {
+  row.each([&](float v) {
     const int d = digit(v);
     if (d < 0) return;
     const unsigned long long w = weigh ? row.fixed(v) : 0;
@@ -360,44 +506,33 @@ __device__ void find_bin(SampleShared& s, const SampleRow<T>& row, bool weigh, u
       ++tail_count;
       tail_mass += w;
     } else {
-      atomicAdd(&s.bins.count[d], 1u);
-      if (w) atomicAdd(&s.bins.mass[d], w);
+      atomicAdd(&bins.count[d], 1u);
+      if (w) atomicAdd(&bins.mass[d], w);
     }
   });
-  tail_count = (uint32_t)block_sum((unsigned long long)tail_count, s.sum_scratch);
-  tail_mass = block_sum(tail_mass, s.sum_scratch);
+  tail_count = (uint32_t)block_sum((unsigned long long)tail_count, s.scan);
+  tail_mass = block_sum(tail_mass, s.scan);
   if (threadIdx.x == 0) {
-    s.bins.count[kBins - 1] = tail_count;
-    s.bins.mass[kBins - 1] = tail_mass;
+    bins.count[kBins - 1] = tail_count;
+    bins.mass[kBins - 1] = tail_mass;
   }
   cluster.sync();
   // Thread i takes bins 4i .. 4i + 3 of all blocks.
   constexpr uint32_t kMine = kBins / kRowThreads;
   uint32_t count[kMine];
-  unsigned long long mass[kMine], sum = 0;
+  unsigned long long mass[kMine], sum = 0, all;
 #pragma unroll
   for (uint32_t j = 0; j < kMine; ++j) {
     count[j] = 0;
     mass[j] = 0;
     for (uint32_t b = 0; b < cluster.num_blocks(); ++b) {
-      const SampleShared* o = cluster.map_shared_rank(&s, b);
-      count[j] += o->bins.count[threadIdx.x * kMine + j];
-      mass[j] += o->bins.mass[threadIdx.x * kMine + j];
+      const Bins* o = cluster.map_shared_rank(&bins, b);
+      count[j] += o->count[threadIdx.x * kMine + j];
+      mass[j] += o->mass[threadIdx.x * kMine + j];
     }
     sum += weigh ? mass[j] : count[j];
   }
-  // Sum of the bins before this thread's.
-  unsigned long long incl = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-    if ((threadIdx.x & 31u) >= (uint32_t)o) incl += up;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31u) == 31u) s.sum_scratch[threadIdx.x >> 5] = incl;
-  __syncthreads();
-  unsigned long long before = incl - sum;
-  for (uint32_t w = 0; w < (threadIdx.x >> 5); ++w) before += s.sum_scratch[w];
+  unsigned long long before = block_scan(sum, s.scan, &all);
 #pragma unroll
   for (uint32_t j = 0; j < kMine; ++j) {
     const unsigned long long in = weigh ? mass[j] : count[j];
@@ -412,22 +547,20 @@ __device__ void find_bin(SampleShared& s, const SampleRow<T>& row, bool weigh, u
 }
 
 // The logit at which the total over the row in descending order reaches `target` (1 <= target <= the
-// total), among logits above `floor`: *edge, and in *ties how many of the tokens with this very logit it
-// takes.
+// total), among logits above `floor`, and how many of the tokens with this very logit it takes.
 template <class T>
-__device__ void find_edge(SampleShared& s, const SampleRow<T>& row, bool weigh, unsigned long long target, float floor, float* edge,
-                          uint32_t* ties) {
+__device__ Kept find_edge(SampleShared& s, Bins& bins, const SampleRow<T>& row, bool weigh, unsigned long long target, float floor) {
   cg::cluster_group cluster = cg::this_cluster();
   // First by distance from the maximum, 1/64 of a temperature a bin and one for all that is 16 below.
   const float scale = fminf((float)(64.0 * row.inv_t), 3e38f);
   auto coarse = [&](float v) { return v == row.m ? 0 : (int)fminf((row.m - v) * scale, (float)(kBins - 1)); };
-  find_bin(s, row, weigh, target, [&](float v) { return v > floor ? coarse(v) : -1; });
+  find_bin(s, bins, row, weigh, target, [&](float v) { return v > floor ? coarse(v) : -1; });
   const int bin = (int)s.found_bin;
   target -= s.found_before;
   uint32_t at = s.found_count;
   // Then by the order keys of the bin's logits, from the first bit in which they differ.
   uint32_t lo = 0xFFFFFFFFu, hi = 0;
-  row.each([&](float v, uint32_t) {
+  row.each([&](float v) {
     if (v > floor && coarse(v) == bin) {
       const uint32_t k = order_key(v);
       lo = min(lo, k);
@@ -446,6 +579,8 @@ __device__ void find_edge(SampleShared& s, const SampleRow<T>& row, bool weigh, 
     atomicMax(&s.key_hi, hi);
   }
   cluster.sync();
+  lo = 0xFFFFFFFFu;
+  hi = 0;
   for (uint32_t b = 0; b < cluster.num_blocks(); ++b) {
     lo = min(lo, cluster.map_shared_rank(&s, b)->key_lo);
     hi = max(hi, cluster.map_shared_rank(&s, b)->key_hi);
@@ -457,7 +592,7 @@ __device__ void find_edge(SampleShared& s, const SampleRow<T>& row, bool weigh, 
     const int step = min(left, 8);
     const int shift = left - step;
     // The largest digit first: digits are counted from the top.
-    find_bin(s, row, weigh, target, [&](float v) {
+    find_bin(s, bins, row, weigh, target, [&](float v) {
       if (!(v > floor) || coarse(v) != bin) return -1;
       const uint32_t k = order_key(v);
       if (left < 32 && (k >> left) != prefix) return -1;
@@ -469,106 +604,76 @@ __device__ void find_edge(SampleShared& s, const SampleRow<T>& row, bool weigh, 
     left = shift;
     __syncthreads();  // found_* is read
   }
-  *edge = key_value(lo == hi ? lo : prefix);
-  const unsigned long long one = row.fixed(*edge);
-  *ties = weigh ? (uint32_t)min((unsigned long long)at, (target + one - 1) / max(one, 1ull)) : (uint32_t)target;
+  Kept kept;
+  kept.edge = key_value(prefix);
+  const unsigned long long one = row.fixed(kept.edge);
+  kept.ties = weigh ? (uint32_t)min((unsigned long long)at, (target + one - 1) / max(one, 1ull)) : (uint32_t)target;
+  return kept;
 }
 
+// The row's token from integer weights of all its tokens, by the whole cluster: into s.token of the block that holds it.
+// `memory`: what the ring left, for the counts.
 template <class T>
-__global__ void __launch_bounds__(kRowThreads)
-    sample_kernel(RowSet x, const float* __restrict__ uniform, ws_sampling sampling, int64_t* __restrict__ tokens,
-                  float* __restrict__ logprobs) {
-  __shared__ SampleShared s;
-  const cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank(), r = blockIdx.x / blocks;
-  float t = sampling.temperature_each ? sampling.temperature_each[r] : sampling.temperature;
-  const float top_p = sampling.top_p_each ? sampling.top_p_each[r] : sampling.top_p;
-  const float min_p = fminf(sampling.min_p_each ? sampling.min_p_each[r] : sampling.min_p, 1.f);
-  int64_t top_k = top_k_of(sampling, r);
-  if (rank == 0 && threadIdx.x == 0) tokens[r] = -1;  // the token's block writes it behind a cluster barrier
-  if (!(t > 0.f)) {
-    t = 1.f;
-    top_k = 1;
-  }
-  if (!(top_p > 0.f)) top_k = 1;
-  const float c = fminf(kLog2e / t, 3e38f);
-  const RowWalk<T> walk(row_ptr<T>(x, r), x.vocab);
-  const uint32_t chunks = (walk.units + kChunkUnits - 1) / kChunkUnits;
-  const uint32_t each = (chunks + blocks - 1) / blocks;
-  const uint32_t chunk0 = min(rank * each, chunks), chunk1 = min(chunk0 + each, chunks);
-  SampleRow<T> row{walk, min(chunk0 * kChunkUnits, walk.units), min(chunk1 * kChunkUnits, walk.units), 0.f, 1.0 / (double)t};
-  const Soft soft = cluster_soft(row_soft(walk, row.first, row.last, c, s.soft_scratch), c, &s.soft_mine);
-  row.m = soft.m;
-  if (soft.m == -INFINITY) {  // the same for the whole cluster
-    if (rank == 0 && threadIdx.x == 0 && logprobs) logprobs[r] = isnan(soft.s) ? NAN : -INFINITY;
-    if (blocks > 1) cluster.sync();
-    return;
-  }
-
-  // The prefix of the order that is kept: all above `edge`, and `ties` of those equal to it.
-  float edge = -INFINITY;
-  uint32_t ties = 0;
-  if (top_k == 1) {
-    edge = soft.m;
-    ties = 1;
-  } else if (top_k > 1 && top_k < (int64_t)x.vocab) {
+__device__ __noinline__ void exact_token(SampleShared& s, void* memory, const SampleRow<T>& row, const SampleSettings& p, uint32_t vocab) {
+  cg::cluster_group cluster = cg::this_cluster();
+  Bins& bins = *reinterpret_cast<Bins*>(memory);
+  Kept kept;
+  if (p.top_k == 1) {
+    kept.edge = row.m;
+    kept.ties = 1;
+  } else if (p.top_k > 1 && p.top_k < (int64_t)vocab) {
     unsigned long long there = 0;
-    row.each([&](float, uint32_t) { ++there; });
-    if (cluster_sum(there, s, row) > (unsigned long long)top_k)
-      find_edge(s, row, false, (unsigned long long)top_k, -INFINITY, &edge, &ties);
+    row.each([&](float) { ++there; });
+    if (cluster_sum(there, s) > (unsigned long long)p.top_k) kept = find_edge(s, bins, row, false, (unsigned long long)p.top_k, -INFINITY);
   }
-  if (top_p < 1.f && !(edge == soft.m && ties == 1)) {
+  if (p.top_p < 1.f && p.top_k != 1) {
     unsigned long long above = 0;
-    row.each([&](float v, uint32_t) { above += v > edge ? row.fixed(v) : 0; });
-    above = cluster_sum(above, s, row);
-    const unsigned long long one = edge > -INFINITY ? row.fixed(edge) : 0;
-    const unsigned long long total = above + one * ties;
-    unsigned long long target = (unsigned long long)ceil((double)top_p * (double)total);
+    row.each([&](float v) { above += v > kept.edge ? row.fixed(v) : 0; });
+    above = cluster_sum(above, s);
+    const unsigned long long one = kept.edge > -INFINITY ? row.fixed(kept.edge) : 0;
+    const unsigned long long total = above + one * kept.ties;
+    unsigned long long target = (unsigned long long)ceil((double)p.top_p * (double)total);
     target = min(max(target, 1ull), total);
     if (target > above)
-      ties = min(ties, (uint32_t)((target - above + one - 1) / max(one, 1ull)));
+      kept.ties = min(kept.ties, (uint32_t)((target - above + one - 1) / max(one, 1ull)));
     else
-      find_edge(s, row, true, target, edge, &edge, &ties);
+      kept = find_edge(s, bins, row, true, target, kept.edge);
   }
 
   // Weights of the tokens kept, in id order: by chunks, then within the chunk that holds the token.
-  // A uniform number of 0 takes the first token of any weight, below 2^-43, too.
-  const double u = (double)uniform[r];
-  const bool first = !(u > 0.0);
-  auto kept = [&](float v) -> unsigned long long {
-    if (min_p > 0.f && !(row.weight(v) >= (double)min_p)) return 0;
-    const unsigned long long w = row.fixed(v);
-    return first && w == 0 && row.weight(v) > 0.0 ? 1 : w;
-  };
-  const unsigned long long one = edge > -INFINITY ? kept(edge) : 0;
+  ChunkSums& sums = *reinterpret_cast<ChunkSums*>(memory);
+  const bool edged = kept.edge > -INFINITY;
+  const unsigned long long one = edged ? row.kept(kept.edge, p) : 0;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t chunk0 = row.first / kChunkUnits;
+  const uint32_t chunk1 = row.first < row.last ? (row.last + kChunkUnits - 1) / kChunkUnits : chunk0;
   unsigned long long mass = 0;
   uint32_t tied = 0;
   __syncthreads();
   for (uint32_t ch = chunk0 + warp; ch < chunk1; ch += kRowWarps) {
     unsigned long long w = 0;
     uint32_t e = 0;
-    for (uint32_t u = ch * kChunkUnits + lane; u < min((ch + 1) * kChunkUnits, walk.units); u += 32) {
-      float f[kUnit];
-      walk.load(u, f);
+    for (uint32_t u = ch * kChunkUnits + lane; u < min((ch + 1) * kChunkUnits, row.last); u += 32) {
+      float f[kUnit<T>];
+      row.walk.load(u, f);
 #pragma unroll
-      for (uint32_t i = 0; i < kUnit; ++i) {
-        if (f[i] > edge) w += kept(f[i]);
-        e += f[i] == edge && edge > -INFINITY;
+      for (uint32_t i = 0; i < kUnit<T>; ++i) {
+        if (f[i] > kept.edge) w += row.kept(f[i], p);
+        e += edged && f[i] == kept.edge;
       }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
     e = __reduce_add_sync(0xFFFFFFFFu, e);
     if (lane == 0) {
-      s.chunks.mass[ch - chunk0] = w;
-      s.chunks.ties[ch - chunk0] = e;
+      sums.mass[ch - chunk0] = w;
+      sums.ties[ch - chunk0] = e;
+      mass += w;
+      tied += e;
     }
-    mass += w;
-    tied += e;
   }
-  mass = block_sum(lane == 0 ? mass : 0ull, s.sum_scratch);
-  tied = (uint32_t)block_sum(lane == 0 ? (unsigned long long)tied : 0ull, s.sum_scratch);
+  mass = block_sum(mass, s.scan);
+  tied = (uint32_t)block_sum((unsigned long long)tied, s.scan);
   if (threadIdx.x == 0) {
     s.mine.mass = mass;
     s.mine.ties = tied;
@@ -576,11 +681,11 @@ __global__ void __launch_bounds__(kRowThreads)
   cluster.sync();
   unsigned long long before = 0, total = 0, mine = 0;
   uint32_t ties_before = 0, seen = 0;
-  for (uint32_t b = 0; b < blocks; ++b) {
+  for (uint32_t b = 0; b < cluster.num_blocks(); ++b) {
     const SampleShared* o = cluster.map_shared_rank(&s, b);
     const uint32_t next = seen + o->mine.ties;
-    const unsigned long long w = o->mine.mass + one * (min(next, ties) - min(seen, ties));
-    if (b == rank) {
+    const unsigned long long w = o->mine.mass + one * (min(next, kept.ties) - min(seen, kept.ties));
+    if (b == cluster.block_rank()) {
       before = total;
       ties_before = seen;
       mine = w;
@@ -588,67 +693,239 @@ __global__ void __launch_bounds__(kRowThreads)
     total += w;
     seen = next;
   }
-  unsigned long long need = !first ? (unsigned long long)fmin(u * (double)total, 9e18) + 1 : 1;
-  need = min(need, total);
-  if (before < need && need <= before + mine && warp == 0) {
-    // 32 chunks at a time.
-    uint32_t ch = chunk0;
-    unsigned long long base = before;
-    uint32_t tie_base = ties_before;
-    for (; ch < chunk1; ch += 32) {
-      const uint32_t q = ch + lane;
-      const uint32_t e = q < chunk1 ? s.chunks.ties[q - chunk0] : 0;
-      uint32_t e_incl = e;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, e_incl, o);
-        if (lane >= (uint32_t)o) e_incl += up;
-      }
-      const uint32_t e0 = tie_base + e_incl - e, e1 = tie_base + e_incl;
-      unsigned long long w = (q < chunk1 ? s.chunks.mass[q - chunk0] : 0ull) + one * (min(e1, ties) - min(e0, ties));
-      const unsigned long long own = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long up = __shfl_up_sync(0xFFFFFFFFu, w, o);
-        if (lane >= (uint32_t)o) w += up;
-      }
-      const uint32_t hit = __ballot_sync(0xFFFFFFFFu, base + w >= need);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        base += __shfl_sync(0xFFFFFFFFu, w - own, l);
-        tie_base = __shfl_sync(0xFFFFFFFFu, e0, l);
-        ch += l;
-        break;
-      }
-      base += __shfl_sync(0xFFFFFFFFu, w, 31);
-      tie_base += __shfl_sync(0xFFFFFFFFu, e_incl, 31);
+  const unsigned long long need = p.need(total);
+  if (before < need && need <= before + mine) {  // the same for the whole block
+    // Thread i takes chunks i * each .. of the block's.
+    const uint32_t n = chunk1 - chunk0, each = (n + kRowThreads - 1) / kRowThreads;
+    const uint32_t c0 = min(threadIdx.x * each, n), c1 = min(c0 + each, n);
+    uint32_t e = 0, all_ties;
+    for (uint32_t c = c0; c < c1; ++c) e += sums.ties[c];
+    uint32_t tie = ties_before + block_scan(e, s.top.sums, &all_ties);
+    const uint32_t tie0 = tie;
+    unsigned long long w = 0, all;
+    for (uint32_t c = c0; c < c1; ++c) {
+      w += sums.mass[c] + one * (min(tie + sums.ties[c], kept.ties) - min(tie, kept.ties));
+      tie += sums.ties[c];
     }
-    for (uint32_t p0 = ch * kChunk; p0 < min((ch + 1) * kChunk, walk.end); p0 += 32) {
-      const uint32_t p = p0 + lane;
-      const float v = p >= walk.head && p < walk.end ? walk.at(p) : -INFINITY;
-      const uint32_t equal = __ballot_sync(0xFFFFFFFFu, v == edge && edge > -INFINITY);
-      const uint32_t nth = tie_base + __popc(equal & ((1u << lane) - 1u));
-      unsigned long long w = 0;
-      if (v > edge) w = kept(v);
-      if (v == edge && edge > -INFINITY && nth < ties) w = one;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long up = __shfl_up_sync(0xFFFFFFFFu, w, o);
-        if (lane >= (uint32_t)o) w += up;
+    unsigned long long at = before + block_scan(w, s.scan, &all);
+    tie = tie0;
+    for (uint32_t c = c0; c < c1; ++c) {
+      const unsigned long long own = sums.mass[c] + one * (min(tie + sums.ties[c], kept.ties) - min(tie, kept.ties));
+      if (at < need && need <= at + own) {
+        s.chunk = chunk0 + c;
+        s.found_before = at;
+        s.found_count = tie;
       }
-      const uint32_t hit = __ballot_sync(0xFFFFFFFFu, base + w >= need);
-      if (hit) {
-        if (lane == (uint32_t)(__ffs(hit) - 1)) {
-          tokens[r] = (int64_t)(p - walk.head);
-          if (logprobs) logprobs[r] = (float)(((double)v - (double)soft.m) * row.inv_t - log((double)soft.s));
-        }
-        break;
-      }
-      base += __shfl_sync(0xFFFFFFFFu, w, 31);
-      tie_base += __popc(equal);
+      at += own;
+      tie += sums.ties[c];
+    }
+    __syncthreads();
+    const unsigned long long base = s.found_before;
+    find_in_chunk(s, row, p, min(s.chunk, chunk1 - 1), kept, s.found_count,
+                  [&](unsigned long long b, unsigned long long a) { return base + b < need && need <= base + a; });
+  }
+  cluster.sync();  // the blocks' shared memory is read until here, and s.token is there
+}
+
+// The token from the row's largest logits, `n` in order in `list`, where they hold all that is kept; false: they may not. The
+// same answer in every block. `all_there`: the row has no others above -inf. total: of the row, in units of
+// the largest weight, off by at most kSumError.
+template <class T>
+__device__ __forceinline__ bool token_of_largest(SampleShared& s, const SampleRow<T>& row, const SampleSettings& p, const uint64_t* list,
+                                                 uint32_t n, bool all_there, uint32_t vocab, double total) {
+  const uint32_t i = threadIdx.x;
+  const bool limited = p.top_k >= 1 && p.top_k < (int64_t)vocab;
+  bool whole = all_there || (limited && p.top_k <= (int64_t)n);  // the list holds all that top-k keeps
+  const uint32_t id = i < n ? 0xFFFFFFFFu - (uint32_t)list[i] : 0xFFFFFFFFu;
+  const float v = i < n ? candidate_value(list[i]) : -INFINITY;
+  const double weight = i < n ? row.weight(v) : 0.0;
+  const unsigned long long fixed = __double2ull_rn(weight * kWeightOne);
+  uint32_t keep = n;
+  if (p.top_p < 1.f && p.top_k != 1) {
+    unsigned long long sum;
+    const unsigned long long cum = block_scan(fixed, s.scan, &sum) + fixed;
+    if (whole) {
+      unsigned long long target = (unsigned long long)ceil((double)p.top_p * (double)sum);
+      target = min(max(target, 1ull), sum);
+      keep = __syncthreads_count(i < n && cum < target) + 1;
+    } else {
+      if (limited) return false;
+      const double target = (double)p.top_p * total * kWeightOne, off = 2 * kSumError * target + 512.0;
+      const uint32_t low = __syncthreads_count(i < n && (double)cum < target - off);
+      const uint32_t high = __syncthreads_count(i < n && (double)cum < target + off);
+      if (low != high || low >= n) return false;
+      keep = low + 1;
+      whole = true;
     }
   }
-  if (blocks > 1) cluster.sync();  // the blocks' shared memory is read until here
+  if (p.min_p > 0.f) {
+    const uint32_t heavy = __syncthreads_count(i < keep && weight >= (double)p.min_p);
+    whole = whole || heavy < keep;
+    keep = heavy;
+  }
+  if (!whole) return false;
+  const unsigned long long w = i < keep ? (p.first() && fixed == 0 && weight > 0.0 ? 1 : fixed) : 0;
+  const unsigned long long sum = block_sum(w, s.scan);
+  const unsigned long long need = p.need(sum);
+  s.weight[i] = w;
+  __syncthreads();
+  if (i < keep) {
+    unsigned long long cum = 0;
+#pragma unroll 4
+    for (uint32_t q = 0; q < keep; ++q) cum += 0xFFFFFFFFu - (uint32_t)list[q] <= id ? s.weight[q] : 0;
+    if (w && cum >= need && cum - w < need) s.token = ((uint64_t)id << 32) | order_key(v);
+  }
+  return true;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kRowThreads, 2)
+    sample_kernel(RowSet x, const float* __restrict__ uniform, ws_sampling sampling, int64_t* __restrict__ tokens,
+                  float* __restrict__ logprobs) {
+  // The ring (then what exact_token counts), (m, s) of the row's chunks, and, where the row has several blocks, what they tell each other.
+  extern __shared__ __align__(16) uint8_t memory[];
+  __shared__ SampleShared s;
+  const RowCluster cluster;
+  cluster.started();
+  const uint32_t r = cluster.row();
+  const SampleSettings p(sampling, uniform, r);
+  const float c = fminf(kLog2e / p.t, 3e38f);
+  const RowWalk<T> walk(row_ptr<T>(x, r), x.vocab);
+  const uint32_t chunks = (walk.units + kChunkUnits - 1) / kChunkUnits;
+  uint32_t chunk0, chunk1;
+  split_units(chunks, cluster.rank, cluster.blocks, chunk0, chunk1);
+  SampleRow<T> row{walk, chunk0 * kChunkUnits, min(chunk1 * kChunkUnits, walk.units), 0.f, 1.0 / (double)p.t};
+  row.first = min(row.first, row.last);
+  float2* soft = reinterpret_cast<float2*>(memory + kTopDepth * kStepBytes);
+  TopTold* told = reinterpret_cast<TopTold*>(soft + ((chunks + 1) & ~1u));
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const bool dropping = (p.top_k >= 1 && p.top_k < (int64_t)x.vocab) || p.top_p < 1.f || p.min_p > 0.f;
+  const uint32_t k = p.top_k >= 1 && p.top_k <= WS_TOP_MAX_K ? (uint32_t)p.top_k : WS_TOP_MAX_K;
+
+  Ring<T, kTopDepth> ring(memory, walk, row.first, row.last);
+  TopCollector<T> top(s.top, k, walk.head);
+  if (threadIdx.x == 0) s.token = ~0ull;
+  for (uint32_t u0 = row.first; u0 < row.last; u0 += Batch<T>::kSpan) {
+    Batch<T> b;
+    ring.read(b);
+    float most[Batch<T>::kUnits], all = -INFINITY;
+#pragma unroll
+    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+      most[j] = unit_max<T>(b.raw[j]);
+      all = fmaxf(all, most[j]);
+    }
+    const float m = key_value(__reduce_max_sync(0xFFFFFFFFu, order_key(all)));
+    float sum = step_sum(b, m, c);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    const uint32_t ch = u0 / kChunkUnits + warp;
+    if (lane == 0 && ch < chunk1) soft[ch] = make_float2(m, sum);
+    if (dropping) top.add(b, most, u0);
+    ring.advance();
+  }
+  if (dropping) top.finish();
+  __syncthreads();
+  const uint64_t* list = s.top.sorted;
+  uint32_t n = dropping ? s.top.sorted_count : 0;
+  if (cluster.blocks > 1) {
+    cluster.ready();
+    for (uint32_t b = 0; b < cluster.blocks; ++b) {
+      if (b == cluster.rank) continue;
+      float2* to = cluster.of(soft, b);
+      for (uint32_t i = chunk0 + threadIdx.x; i < chunk1; i += kRowThreads) to[i] = soft[i];
+    }
+    if (dropping) tell_top(cluster, s.top, told);
+    cluster.told();
+    if (dropping) {
+      const uint32_t own = n;
+      n = 0;
+      for (uint32_t b = 0; b < cluster.blocks; ++b) n += told->counts[b];
+      if (threadIdx.x < own) {
+        const uint64_t v = s.top.sorted[threadIdx.x];
+        const uint32_t place = cluster_place(cluster, *told, threadIdx.x, v);
+        if (place < k)
+          for (uint32_t b = 0; b < cluster.blocks; ++b) cluster.of(s.merged, b)[place] = v;
+      }
+      cluster.told();
+      list = s.merged;
+    }
+  }
+  const bool all_there = n < k;
+  n = min(n, k);
+
+  // The row's maximum and total from its chunks', the same in every block.
+  const uint32_t each = (chunks + kRowThreads - 1) / kRowThreads;
+  const uint32_t c0 = min(threadIdx.x * each, chunks), c1 = min(c0 + each, chunks);
+  float m = -INFINITY;
+  for (uint32_t i = c0; i < c1; ++i) m = fmaxf(m, soft[i].x);
+  m = block_max(m, reinterpret_cast<float*>(s.sums));
+  row.m = m;
+  // 2^((x - m) c) of a chunk in 64 bits, with the c that its sum has.
+  auto chunk_sum = [&](uint32_t i) {
+    const float2 t = soft[i];
+    return t.x == -INFINITY ? (double)t.y : (double)t.y * (t.x == m ? 1.0 : exp2(((double)t.x - (double)m) * (double)c));
+  };
+  double mine = 0.0, total;
+  for (uint32_t i = c0; i < c1; ++i) mine += chunk_sum(i);
+  const double before = block_scan(mine, s.sums, &total);
+  if (m == -INFINITY) {  // the same for the whole cluster
+    if (cluster.rank == 0 && threadIdx.x == 0) {
+      tokens[r] = -1;
+      if (logprobs) logprobs[r] = isnan(total) ? NAN : -INFINITY;
+    }
+    return;
+  }
+
+  // A total that is no finite number (NaN or +inf logits) and a factor that has left fp32's range leave it to exact_token.
+  bool decided = false;
+  if (dropping && p.top_k == 1) {
+    if (threadIdx.x == 0) s.token = ((uint64_t)(0xFFFFFFFFu - (uint32_t)list[0]) << 32) | (list[0] >> 32);
+    decided = true;
+  } else if (isfinite(total) && c < 1e30f) {
+    if (dropping) {
+      decided = token_of_largest(s, row, p, list, n, all_there, x.vocab, total);
+    } else if (!p.first()) {
+      const double target = p.u * total;
+      if (threadIdx.x == 0) s.chunk = chunks;
+      __syncthreads();
+      if (before <= target && target < before + mine) {
+        double at = before;
+        for (uint32_t i = c0; i < c1; ++i) {
+          const double own = chunk_sum(i);
+          if (at <= target && target < at + own) {
+            s.chunk = i;
+            s.chunk_before = at;
+          }
+          at += own;
+        }
+      }
+      __syncthreads();
+      if (s.chunk < chunks) {
+        const double base = s.chunk_before * kWeightOne, goal = target * kWeightOne, off = 2 * kSumError * goal + 2048.0;
+        find_in_chunk(s, row, p, s.chunk, Kept{}, 0, [&](unsigned long long b, unsigned long long a) {
+          return base + (double)b < goal - off && base + (double)a > goal + off;
+        });
+        __syncthreads();
+        decided = s.token != ~0ull;
+      }
+    }
+  }
+  const bool here = decided;
+  if (!decided) {
+    __syncthreads();
+    exact_token(s, memory, row, p, x.vocab);
+  } else {
+    __syncthreads();
+  }
+  // Decided above, every block has the token; exact_token leaves it in the block that holds it (or in none, if logits
+  // change while they are read).
+  if (threadIdx.x == 0) {
+    const uint64_t token = s.token;
+    if (here ? cluster.rank == 0 : token != ~0ull) {
+      tokens[r] = (int64_t)(token >> 32);
+      if (logprobs) logprobs[r] = (float)(((double)key_value((uint32_t)token) - (double)m) * row.inv_t - log(total));
+    }
+  }
 }
 
 int fail(int code, const std::string& msg) {
@@ -681,8 +958,9 @@ extern "C" int ws_top_logprobs(const ws_rows* logits, uint32_t k, float temperat
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(top_kernel<T>, x.rows, blocks_a_row(x.rows, x.set.vocab / kUnit), stream, x.set, k, kLog2e / temperature, 1.f / temperature, ids,
-                           logprobs);
+        const uint32_t blocks = blocks_a_row(x);
+        return launch_rows<top_kernel<T>>(x.rows, blocks, kTopDepth * kStepBytes + (blocks > 1 ? sizeof(TopTold) : 0), device, stream,
+                                          x.set, k, kLog2e / temperature, 1.f / temperature, ids, logprobs);
       });
     return done(e, "top log-probabilities");
   });
@@ -703,7 +981,10 @@ extern "C" int ws_sample(const ws_rows* logits, const float* uniform, const ws_s
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(sample_kernel<T>, x.rows, blocks_a_row(x.rows, x.set.vocab / kUnit), stream, x.set, uniform, *sampling, tokens, logprobs);
+        const uint32_t blocks = blocks_a_row(x);
+        const uint32_t chunks = (x.set.vocab + 2 * kUnit<T> - 2) / kChunk<T> + 1;  // at most, with the row's head
+        return launch_rows<sample_kernel<T>>(x.rows, blocks, kTopDepth * kStepBytes + ((chunks + 1) & ~1u) * sizeof(float2) + (blocks > 1 ? sizeof(TopTold) : 0),
+                                             device, stream, x.set, uniform, *sampling, tokens, logprobs);
       });
     return done(e, "sample");
   });

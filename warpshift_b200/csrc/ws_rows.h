@@ -3,10 +3,9 @@
 //
 // A row has V contiguous elements. It is walked in "aligned positions": position
 // p = 0 is the last 16-byte boundary at or before the row, so element i sits at
-// p = i + head, with head < 8 elements, and every unit of 8 positions is one
-// (16-bit types) or two (fp32) aligned 16-byte loads whatever the row's own
-// alignment. The units that reach over either end of the row are loaded element by
-// element; nothing outside the row is read.
+// p = i + head, and every unit of 16 bytes (8 or 4 positions) is one aligned load
+// whatever the row's own alignment. The units that reach over either end of the row
+// are loaded element by element; nothing outside the row is read.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -15,13 +14,16 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/warpshift_b200.h"
 
 namespace ws {
 
 constexpr uint32_t kRowThreads = 256;
 constexpr uint32_t kRowWarps = kRowThreads / 32;
-constexpr uint32_t kUnit = 8;  // elements of one load step of a thread
+template <class T>
+constexpr uint32_t kUnit = 16 / sizeof(T);  // elements of a 16-byte unit
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Device copy of ws_rows (strides in elements).
@@ -55,18 +57,12 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <>
 __device__ __forceinline__ float from_float<float>(float x) { return x; }
 
-// Eight consecutive elements as they lie in memory: one 16-byte word for the
-// 16-bit types, two for fp32.
+// A unit's elements, as they lie in memory, as fp32; and back, rounded.
 template <class T>
-struct Raw {
-  uint4 v[sizeof(T) / 2];
-};
-
-template <class T>
-__device__ __forceinline__ void unpack(const Raw<T>& r, float (&f)[kUnit]);
+__device__ __forceinline__ void unpack(const uint4& r, float (&f)[kUnit<T>]);
 template <>
-__device__ __forceinline__ void unpack<__nv_bfloat16>(const Raw<__nv_bfloat16>& r, float (&f)[kUnit]) {
-  const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+__device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& r, float (&f)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     f[2 * i] = __uint_as_float(w[i] << 16);
@@ -74,8 +70,8 @@ __device__ __forceinline__ void unpack<__nv_bfloat16>(const Raw<__nv_bfloat16>& 
   }
 }
 template <>
-__device__ __forceinline__ void unpack<__half>(const Raw<__half>& r, float (&f)[kUnit]) {
-  const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+__device__ __forceinline__ void unpack<__half>(const uint4& r, float (&f)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -84,40 +80,38 @@ __device__ __forceinline__ void unpack<__half>(const Raw<__half>& r, float (&f)[
   }
 }
 template <>
-__device__ __forceinline__ void unpack<float>(const Raw<float>& r, float (&f)[kUnit]) {
-  const uint32_t w[8] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w, r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+__device__ __forceinline__ void unpack<float>(const uint4& r, float (&f)[4]) {
+  f[0] = __uint_as_float(r.x);
+  f[1] = __uint_as_float(r.y);
+  f[2] = __uint_as_float(r.z);
+  f[3] = __uint_as_float(r.w);
 }
 
 template <class T>
-__device__ __forceinline__ Raw<T> pack(const float (&f)[kUnit]);
+__device__ __forceinline__ uint4 pack(const float (&f)[kUnit<T>]);
 template <>
-__device__ __forceinline__ Raw<__nv_bfloat16> pack<__nv_bfloat16>(const float (&f)[kUnit]) {
+__device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float (&f)[8]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
     w[i] = *reinterpret_cast<const uint32_t*>(&p);
   }
-  return {{make_uint4(w[0], w[1], w[2], w[3])}};
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <>
-__device__ __forceinline__ Raw<__half> pack<__half>(const float (&f)[kUnit]) {
+__device__ __forceinline__ uint4 pack<__half>(const float (&f)[8]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
     w[i] = *reinterpret_cast<const uint32_t*>(&p);
   }
-  return {{make_uint4(w[0], w[1], w[2], w[3])}};
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <>
-__device__ __forceinline__ Raw<float> pack<float>(const float (&f)[kUnit]) {
-  Raw<float> r;
-  r.v[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-  r.v[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
-  return r;
+__device__ __forceinline__ uint4 pack<float>(const float (&f)[4]) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
 }
 
 // One row as a CTA walks it. first/last: its units [first, last) of the row's
@@ -131,86 +125,111 @@ struct RowWalk {
     head = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T);
     aligned = row - head;
     end = head + vocab;
-    units = (end + kUnit - 1) / kUnit;
+    units = (end + kUnit<T> - 1) / kUnit<T>;
   }
-  // Whether all eight positions of unit u belong to the row.
-  __device__ __forceinline__ bool whole(uint32_t u) const { return u * kUnit >= head && (u + 1) * kUnit <= end; }
+  // Whether all positions of unit u belong to the row.
+  __device__ __forceinline__ bool whole(uint32_t u) const { return u * kUnit<T> >= head && (u + 1) * kUnit<T> <= end; }
   __device__ __forceinline__ float at(uint32_t p) const { return to_float(aligned[p]); }
   // Unit u; positions outside the row read as -inf.
-  __device__ __forceinline__ void load(uint32_t u, float (&f)[kUnit]) const {
+  __device__ __forceinline__ void load(uint32_t u, float (&f)[kUnit<T>]) const {
     if (whole(u)) {
-      Raw<T> r;
-      const uint4* v = reinterpret_cast<const uint4*>(aligned + (size_t)u * kUnit);
-#pragma unroll
-      for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.v[i] = __ldg(v + i);
-      unpack<T>(r, f);
+      unpack<T>(__ldg(reinterpret_cast<const uint4*>(aligned) + u), f);
     } else {
 #pragma unroll
-      for (uint32_t i = 0; i < kUnit; ++i) {
-        const uint32_t p = u * kUnit + i;
+      for (uint32_t i = 0; i < kUnit<T>; ++i) {
+        const uint32_t p = u * kUnit<T> + i;
         f[i] = (p >= head && p < end) ? at(p) : -INFINITY;
       }
     }
   }
 };
 
-// 16 bytes that are read once: not kept in L1.
-__device__ __forceinline__ uint4 load16(const void* p) {
-  uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
-// -inf in every element of a word.
-template <class T>
-constexpr uint32_t kNegInf = 0xFF800000u;
-template <>
-constexpr uint32_t kNegInf<__nv_bfloat16> = 0xFF80FF80u;
-template <>
-constexpr uint32_t kNegInf<__half> = 0xFC00FC00u;
-
-// What a block reads of a row in one step: kBatch units from each thread, thread t's j-th one at
-// u0 + j * kRowThreads + t. 64 bytes a thread in flight for either element size.
+// What a thread takes of a row in one step: kUnits units.
 template <class T>
 struct Batch {
-  static constexpr uint32_t kUnits = 8 / sizeof(T);
-  static constexpr uint32_t kSpan = kUnits * kRowThreads;  // units of the block's step
-  Raw<T> raw[kUnits];
+  static constexpr uint32_t kUnits = 4;
+  static constexpr uint32_t kWarpSpan = kUnits * 32;          // units of a warp's step, contiguous
+  static constexpr uint32_t kSpan = kUnits * kRowThreads;     // units of the block's step
+  uint4 raw[kUnits];
 
-  // Units [u0, u0 + kSpan) up to `last`; what lies outside is -inf.
-  __device__ __forceinline__ void load(const RowWalk<T>& walk, uint32_t u0, uint32_t last) {
-    if (u0 * kUnit >= walk.head && u0 + kSpan <= last && (u0 + kSpan) * kUnit <= walk.end) {
-      const T* p = walk.aligned + (size_t)(u0 + threadIdx.x) * kUnit;
+  // The thread's j-th unit in the block's step that begins at unit u0.
+  static __device__ __forceinline__ uint32_t unit(uint32_t u0, uint32_t j) {
+    return u0 + (threadIdx.x >> 5) * kWarpSpan + j * 32 + (threadIdx.x & 31u);
+  }
+};
+
+// The way of a row's units through shared memory: kDepth steps of asynchronous 16-byte copies in flight. Every
+// thread copies and reads units of its own, so that nothing waits for another
+// thread. Bytes in flight are what a block that shares its SM with two or three others needs to
+// keep HBM busy (about 44 bytes a ns for an SM, for about a microsecond), without
+// registers to hold them.
+constexpr uint32_t kStepBytes = 64 * kRowThreads;
+
+template <class T, uint32_t kDepth>
+class Ring {
+ public:
+  using B = Batch<T>;
+
+  // `memory`: kDepth * kStepBytes, 16-byte aligned. Units [first, last) are read.
+  __device__ __forceinline__ Ring(void* memory, const RowWalk<T>& walk, uint32_t first, uint32_t last)
+      : walk_(walk), last_(last), ahead_(first), slot_(0) {
+    mine_ = (uint32_t)__cvta_generic_to_shared(memory) + threadIdx.x * 16;
 #pragma unroll
-      for (uint32_t j = 0; j < kUnits; ++j)
+    for (uint32_t d = 0; d < kDepth; ++d) fill(d);
+  }
+  // Every copy has landed; the memory may be used for something else behind a barrier.
+  static __device__ __forceinline__ void drain() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+  // The next step's units, those outside the row or the range as -inf.
+  __device__ __forceinline__ void read(B& b) const {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    fetch(slot_, b);
+  }
+  // Step `slot` of the first kDepth, which stays where it is as long as no later step is copied over it.
+  __device__ __forceinline__ void again(uint32_t slot, B& b) const { fetch(slot, b); }
+  // To the step after it; to be called when what read() gave has been used.
+  __device__ __forceinline__ void advance() {
+    fill(slot_);
+    slot_ = slot_ + 1 == kDepth ? 0 : slot_ + 1;
+  }
+
+ private:
+  __device__ __forceinline__ uint32_t at(uint32_t slot, uint32_t j) const { return mine_ + slot * kStepBytes + j * (kRowThreads * 16); }
+  __device__ __forceinline__ void fetch(uint32_t slot, B& b) const {
 #pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) / 2; ++i) raw[j].v[i] = load16(p + j * kRowThreads * kUnit + i * (16 / sizeof(T)));
-      return;
+    for (uint32_t j = 0; j < B::kUnits; ++j) {
+      uint4& v = b.raw[j];
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at(slot, j)) : "memory");
     }
+  }
+  __device__ __forceinline__ void fill(uint32_t slot) {
+    const uint32_t u0 = ahead_;
+    if (u0 < last_) {
+      const bool inside = u0 * kUnit<T> >= walk_.head && u0 + B::kSpan <= last_ && (u0 + B::kSpan) * kUnit<T> <= walk_.end;
 #pragma unroll
-    for (uint32_t j = 0; j < kUnits; ++j) {
-      const uint32_t u = u0 + j * kRowThreads + threadIdx.x;
-      if (u < last && walk.whole(u)) {
+      for (uint32_t j = 0; j < B::kUnits; ++j) {
+        const uint32_t u = B::unit(u0, j);
+        if (inside || (u < last_ && walk_.whole(u))) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(slot, j)), "l"(reinterpret_cast<const uint4*>(walk_.aligned) + u)
+                       : "memory");
+        } else {
+          float f[kUnit<T>];
 #pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) / 2; ++i)
-          raw[j].v[i] = load16(walk.aligned + (size_t)u * kUnit + i * (16 / sizeof(T)));
-      } else {
-        float f[kUnit];
-#pragma unroll
-        for (uint32_t i = 0; i < kUnit; ++i) {
-          const uint32_t p = u * kUnit + i;
-          f[i] = u < last && p >= walk.head && p < walk.end ? walk.at(p) : -INFINITY;
+          for (uint32_t i = 0; i < kUnit<T>; ++i) {
+            const uint32_t p = u * kUnit<T> + i;
+            f[i] = u < last_ && p >= walk_.head && p < walk_.end ? walk_.at(p) : -INFINITY;
+          }
+          const uint4 r = pack<T>(f);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at(slot, j)), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
         }
-        raw[j] = pack<T>(f);
       }
     }
+    ahead_ = u0 + B::kSpan;
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (uint32_t j = 0; j < kUnits; ++j)
-#pragma unroll
-      for (uint32_t i = 0; i < sizeof(T) / 2; ++i) raw[j].v[i] = make_uint4(kNegInf<T>, kNegInf<T>, kNegInf<T>, kNegInf<T>);
-  }
+
+  const RowWalk<T>& walk_;
+  uint32_t last_, ahead_, slot_, mine_;
 };
 
 // Pairs of fp32 in one instruction.
@@ -235,6 +254,36 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return v;
 }
 
+// Floats as integers of the same order (-0 is taken as +0 first, so that equal
+// logits have equal keys).
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+// Sum of 2^((x - m) c) over a thread's units of a step (m = -inf: all of them are -inf, and the sum is 0).
+template <class T>
+__device__ __forceinline__ float step_sum(const Batch<T>& b, float m, float c) {
+  const float base = m == -INFINITY ? 0.f : m;
+  const uint64_t nb = pair(-base, -base), cc = pair(c, c);
+  uint64_t sum = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+    float f[kUnit<T>];
+    unpack<T>(b.raw[j], f);
+#pragma unroll
+    for (uint32_t i = 0; i < kUnit<T>; i += 2) {
+      const float2 e = unpair(mul2(add2(pair(f[i], f[i + 1]), nb), cc));
+      sum = add2(sum, pair(ex2(e.x), ex2(e.y)));
+    }
+  }
+  const float2 t = unpair(sum);
+  return t.x + t.y;
+}
+
 // Running maximum m and sum s of 2^((x - m) c), c = log2(e) / temperature. The
 // difference x - m is taken before the product, so logits of any size (a mask of
 // the type's lowest value, say) give exponents that are exact near the maximum.
@@ -250,21 +299,7 @@ struct Soft {
       s *= ex2((m - top) * c);
       m = top;
     }
-    const float base = m == -INFINITY ? 0.f : m;
-    const uint64_t nb = pair(-base, -base), cc = pair(c, c);
-    uint64_t sum = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
-      float f[kUnit];
-      unpack<T>(b.raw[j], f);
-#pragma unroll
-      for (uint32_t i = 0; i < kUnit; i += 2) {
-        const float2 e = unpair(mul2(add2(pair(f[i], f[i + 1]), nb), cc));
-        sum = add2(sum, pair(ex2(e.x), ex2(e.y)));
-      }
-    }
-    const float2 t = unpair(sum);
-    s += t.x + t.y;
+    s += step_sum(b, m, c);
   }
   __device__ __forceinline__ void merge(float m2, float s2, float c) {
     const float top = fmaxf(m, m2);
@@ -288,22 +323,47 @@ __device__ __forceinline__ V block_sum(V v, V* scratch) {
   return t;
 }
 
-// The block's statistics from its threads', in a fixed order; every thread gets them.
+// The block's statistics from its threads', in a fixed order; every thread gets them. The maximum
+// first, so that a thread's sum is scaled once.
 __device__ __forceinline__ Soft block_soft(Soft t, float c, float2* scratch) {
+  const float top = key_value(__reduce_max_sync(0xFFFFFFFFu, order_key(t.m)));
+  t.s *= t.m == top ? 1.f : ex2((t.m - top) * c);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xFFFFFFFFu, t.m, o), s2 = __shfl_xor_sync(0xFFFFFFFFu, t.s, o);
-    t.merge(m2, s2, c);
-  }
+  for (int o = 16; o > 0; o >>= 1) t.s += __shfl_xor_sync(0xFFFFFFFFu, t.s, o);
   __syncthreads();
-  if ((threadIdx.x & 31u) == 0) scratch[threadIdx.x >> 5] = make_float2(t.m, t.s);
+  if ((threadIdx.x & 31u) == 0) scratch[threadIdx.x >> 5] = make_float2(top, t.s);
   __syncthreads();
   Soft r;
   r.m = scratch[0].x;
-  r.s = scratch[0].y;
 #pragma unroll
-  for (uint32_t w = 1; w < kRowWarps; ++w) r.merge(scratch[w].x, scratch[w].y, c);
+  for (uint32_t w = 1; w < kRowWarps; ++w) r.m = fmaxf(r.m, scratch[w].x);
+#pragma unroll
+  for (uint32_t w = 0; w < kRowWarps; ++w) r.s += scratch[w].y * (scratch[w].x == r.m ? 1.f : ex2((scratch[w].x - r.m) * c));
   return r;
+}
+
+// Sum over the threads before this one, in a fixed order; *total: over all.
+template <class V>
+__device__ __forceinline__ V block_scan(V v, V* scratch, V* total) {
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+  V incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    if (lane >= (uint32_t)o) incl += up;
+  }
+  __syncthreads();
+  if (lane == 31u) scratch[warp] = incl;
+  __syncthreads();
+  V before = 0, all = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kRowWarps; ++w) {
+    if (w == warp) before = all;
+    all += scratch[w];
+  }
+  *total = all;
+  const V excl = __shfl_up_sync(0xFFFFFFFFu, incl, 1);
+  return before + (lane ? excl : V(0));
 }
 
 // The largest of the block's values; every thread gets it.
@@ -319,60 +379,75 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
   return t;
 }
 
-// The row's statistics from those of the cluster's blocks, which all get them. `mine`
-// is the block's slot, which no block writes again before the next cluster barrier.
-__device__ __forceinline__ Soft cluster_soft(const Soft& block, float c, float2* mine) {
-  namespace cg = cooperative_groups;
-  cg::cluster_group cluster = cg::this_cluster();
-  if (cluster.num_blocks() == 1) return block;
-  if (threadIdx.x == 0) *mine = make_float2(block.m, block.s);
-  cluster.sync();
-  Soft r;
-  for (uint32_t b = 0; b < cluster.num_blocks(); ++b) {
-    const float2 v = *cluster.map_shared_rank(mine, b);
-    if (b == 0) {
-      r.m = v.x;
-      r.s = v.y;
+// The blocks of a cluster (1, 2, 4 or 8) share a row and tell each other what they found by storing into each
+// other's shared memory, so that a block may leave as soon as it has what it needs:
+//   started() at the kernel's begin; ready() before the first store into another block;
+//   told() behind the stores: from then on every block's stores to this one are there.
+class RowCluster {
+ public:
+  static constexpr uint32_t kMost = 8;
+
+  __device__ __forceinline__ RowCluster() : blocks(cooperative_groups::this_cluster().num_blocks()), rank(cooperative_groups::this_cluster().block_rank()) {}
+  __device__ __forceinline__ void started() const {
+    if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  }
+  __device__ __forceinline__ void ready() const {
+    if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  __device__ __forceinline__ void told() const {
+    if (blocks > 1) {
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     } else {
-      r.merge(v.x, v.y, c);
+      __syncthreads();
     }
   }
+  // `p` of this block's shared memory, in block b's.
+  template <class V>
+  __device__ __forceinline__ V* of(V* p, uint32_t b) const {
+    return cooperative_groups::this_cluster().map_shared_rank(p, b);
+  }
+  __device__ __forceinline__ uint32_t row() const { return blockIdx.x / blocks; }
+
+  const uint32_t blocks, rank;
+};
+
+// The row's statistics from those of the cluster's blocks, which all get them; between ready() and told().
+__device__ __forceinline__ void tell_soft(const RowCluster& cluster, const Soft& block, float2* slots) {
+  if (threadIdx.x < cluster.blocks) *cluster.of(slots + cluster.rank, threadIdx.x) = make_float2(block.m, block.s);
+}
+__device__ __forceinline__ Soft told_soft(const RowCluster& cluster, float c, const float2* slots) {
+  Soft r;
+  r.m = slots[0].x;
+  r.s = slots[0].y;
+  for (uint32_t b = 1; b < cluster.blocks; ++b) r.merge(slots[b].x, slots[b].y, c);
   return r;
 }
 
 template <class T>
-__device__ __forceinline__ float unit_max(const Raw<T>& r) {
-  float f[kUnit];
+__device__ __forceinline__ float unit_max(const uint4& r) {
+  float f[kUnit<T>];
   unpack<T>(r, f);
-  return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+  float top = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+#pragma unroll
+  for (uint32_t i = 4; i < kUnit<T>; i += 2) top = fmaxf(top, fmaxf(f[i], f[i + 1]));
+  return top;
 }
 
-// Statistics of units [first, last) of a row, for the whole block. The loads of a step are in flight while
-// the step before is summed up.
-template <class T>
-__device__ __forceinline__ Soft row_soft(const RowWalk<T>& walk, uint32_t first, uint32_t last, float c, float2* scratch) {
+// Statistics of the units that `ring` reads, for the whole block.
+template <class T, uint32_t kDepth>
+__device__ __forceinline__ Soft row_soft(Ring<T, kDepth>& ring, uint32_t first, uint32_t last, float c, float2* scratch) {
   Soft soft;
-  Batch<T> next;
-  if (first < last) next.load(walk, first, last);
   for (uint32_t u = first; u < last; u += Batch<T>::kSpan) {
-    const Batch<T> now = next;
-    if (u + Batch<T>::kSpan < last) next.load(walk, u + Batch<T>::kSpan, last);
-    float top = unit_max<T>(now.raw[0]);
+    Batch<T> b;
+    ring.read(b);
+    float top = unit_max<T>(b.raw[0]);
 #pragma unroll
-    for (uint32_t j = 1; j < Batch<T>::kUnits; ++j) top = fmaxf(top, unit_max<T>(now.raw[j]));
-    soft.add(now, top, c);
+    for (uint32_t j = 1; j < Batch<T>::kUnits; ++j) top = fmaxf(top, unit_max<T>(b.raw[j]));
+    soft.add(b, top, c);
+    ring.advance();
   }
   return block_soft(soft, c, scratch);
-}
-
-// Floats as integers of the same order (-0 is taken as +0 first, so that equal
-// logits have equal keys).
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t b = __float_as_uint(x + 0.f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float key_value(uint32_t k) {
-  return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
 // Units of the row that block `rank` of `blocks` walks.
@@ -425,19 +500,32 @@ cudaError_t by_type(int dtype, F&& f) {
   }
 }
 
-// How many blocks (a cluster: 1, 2, 4 or 8) share each of `rows` rows of `units` units.
-inline uint32_t blocks_a_row(uint32_t rows, uint32_t units) {
+// How many blocks (a cluster: 1, 2, 4 or 8) share each row.
+inline uint32_t blocks_a_row(const RowArgs& x) {
+  const uint32_t bytes = x.set.vocab * (x.dtype == WS_DTYPE_FP32 ? 4u : 2u);
   uint32_t c = 1;
-  while (c < 8 && (uint64_t)rows * c * 2 <= 592 && units / c >= 512) c *= 2;
+  while (c < 8 && (uint64_t)x.rows * c * 2 <= 592 && bytes / c >= 8192) c *= 2;
   return c;
 }
 
-// Launches `rows` clusters of `cluster` blocks of kRowThreads threads.
-template <class... P, class... A>
-cudaError_t launch_rows(void (*kernel)(P...), uint32_t rows, uint32_t cluster, void* stream, A... args) {
+// Launches `rows` clusters of `cluster` blocks of kRowThreads threads with `smem` bytes of dynamic shared memory each.
+template <auto kernel, class... A>
+cudaError_t launch_rows(uint32_t rows, uint32_t cluster, size_t smem, int device, void* stream, A... args) {
+  // More than 48 KiB of shared memory in all has to be asked for, once for a kernel and device.
+  static std::atomic<uint64_t> told{0};
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (!(told.load(std::memory_order_relaxed) & bit)) {
+    cudaFuncAttributes own;
+    cudaError_t e = cudaFuncGetAttributes(&own, kernel);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)own.sharedSizeBytes);
+    if (e != cudaSuccess) return e;
+    told.fetch_or(bit);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * cluster);
   cfg.blockDim = dim3(kRowThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -446,7 +534,7 @@ cudaError_t launch_rows(void (*kernel)(P...), uint32_t rows, uint32_t cluster, v
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 }  // namespace ws

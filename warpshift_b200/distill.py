@@ -52,17 +52,46 @@ def _record(logits, ids, logprobs, weights, temperature, tail):
         weights = per_row(weights, "weights", logits, (torch.float32,))
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError(f"temperature must be from 1e-6 to 1e6, not {temperature}")
-    record = _lib.Teacher(ids.data_ptr(), logprobs.data_ptr(), None if weights is None else weights.data_ptr(), k,
-                          ids.dtype == torch.int32, _lib.TAILS[tail], temperature)
-    return record, (ids, logprobs, weights)
+    return _teacher(ids, logprobs, weights, temperature, tail), (ids, logprobs, weights)
+
+
+def _teacher(ids, logprobs, weights, temperature, tail):
+    return _lib.Teacher(ids.data_ptr(), logprobs.data_ptr(), None if weights is None else weights.data_ptr(), ids.shape[-1],
+                        ids.dtype == torch.int32, _lib.TAILS[tail], temperature)
 
 
 def _grad_like(logits: torch.Tensor, rows: _lib.Rows) -> torch.Tensor:
     """Room for the gradient. Rows that lie a little apart (a padded vocabulary) stay so: a gradient row on the same
     offset from a 16-byte boundary as its logits is written with the widest stores."""
     if logits.dim() == 2 and rows.vocab < rows.stride_inner <= rows.vocab + rows.vocab // 8:
-        return torch.empty((rows.rows, rows.stride_inner), dtype=logits.dtype, device=logits.device)[:, : rows.vocab]
-    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return logits.new_empty((rows.rows, rows.stride_inner))[:, : rows.vocab]
+    return logits.new_empty(logits.shape)
+
+
+def _backward(ctx, grad_loss):
+    logits, ids, logprobs, weights, stats = ctx.saved_tensors
+    # Anew from the saved tensors: hooks on them (offloading, say) may have put them elsewhere.
+    rows = rows_of(logits)
+    record = _teacher(ids, logprobs, weights, *ctx.settings)
+    # One g for each row by the strides of the logits' two row dimensions; a sum's or a mean's gradient has strides of 0.
+    if grad_loss.dtype != torch.float32:
+        grad_loss = grad_loss.float()
+    if logits.dim() == 2:
+        outer, inner = 0, grad_loss.stride(0)
+    elif all(s == 0 for s in grad_loss.stride()):
+        outer = inner = 0
+    else:
+        grad_loss = grad_loss.contiguous()
+        outer, inner = rows.inner, 1
+    grad = _grad_like(logits, rows)
+    out = rows_of(grad, "gradient")
+    index = logits.get_device()
+    _lib.check(_lib.load().ws_distill_backward(byref(rows), byref(record), stats.data_ptr(), grad_loss.data_ptr(), outer, inner,
+                                               byref(out), index, stream_of(index)))
+    return grad, None, None, None, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 class _TopLogprobLoss(torch.autograd.Function):
@@ -70,36 +99,19 @@ class _TopLogprobLoss(torch.autograd.Function):
     def forward(ctx, logits, ids, logprobs, weights, temperature, tail):
         rows = rows_of(logits)
         record, (ids, logprobs, weights) = _record(logits, ids, logprobs, weights, temperature, tail)
-        device = device_of(logits)
-        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
-        stats = torch.empty((rows.rows, _lib.WS_DISTILL_STATS), dtype=torch.float32, device=device)
-        _lib.check(_lib.load().ws_distill_forward(byref(rows), byref(record), loss.data_ptr(), stats.data_ptr(), device.index,
-                                                  stream_of(device)))
+        index = device_of(logits)
+        loss = logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+        stats = logits.new_empty((rows.rows, _lib.WS_DISTILL_STATS), dtype=torch.float32)
+        _lib.check(_lib.load().ws_distill_forward(byref(rows), byref(record), loss.data_ptr(), stats.data_ptr(), index,
+                                                  stream_of(index)))
         ctx.save_for_backward(logits, ids, logprobs, weights, stats)
         ctx.settings = temperature, tail
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        logits, ids, logprobs, weights, stats = ctx.saved_tensors
-        rows = rows_of(logits)
-        record, _ = _record(logits, ids, logprobs, weights, *ctx.settings)
-        # One g for each row by the strides of the logits' two row dimensions; a sum's or a mean's gradient has strides of 0.
-        if grad_loss.dtype != torch.float32:
-            grad_loss = grad_loss.float()
-        if logits.dim() == 2:
-            outer, inner = 0, grad_loss.stride(0)
-        elif all(s == 0 for s in grad_loss.stride()):
-            outer = inner = 0
-        else:
-            grad_loss = grad_loss.contiguous()
-            outer, inner = rows.inner, 1
-        grad = _grad_like(logits, rows)
-        out = rows_of(grad, "gradient")
-        _lib.check(_lib.load().ws_distill_backward(byref(rows), byref(record), stats.data_ptr(), grad_loss.data_ptr(), outer, inner,
-                                                   byref(out), logits.device.index, stream_of(logits.device)))
-        return grad, None, None, None, None, None
+        # Under create_graph the result is marked as differentiable no further, which costs 10 us that other calls need not pay.
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_loss)
 
 
 def top_logprob_loss(
@@ -121,7 +133,6 @@ def top_logprob_loss(
     return _TopLogprobLoss.apply(logits, ids, logprobs, weights, temperature, tail)
 
 
-@torch.no_grad()
 def top_logprob_loss_and_grad(
     logits: torch.Tensor,
     ids: torch.Tensor,
@@ -138,9 +149,9 @@ def top_logprob_loss_and_grad(
     """
     rows = rows_of(logits)
     record, keep = _record(logits, ids, logprobs, weights, temperature, tail)
-    device = device_of(logits)
-    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
+    index = device_of(logits)
+    loss = logits.new_empty(logits.shape[:-1], dtype=torch.float32)
     grad = _grad_like(logits, rows)
     out = rows_of(grad, "gradient")
-    _lib.check(_lib.load().ws_distill_step(byref(rows), byref(record), loss.data_ptr(), byref(out), device.index, stream_of(device)))
+    _lib.check(_lib.load().ws_distill_step(byref(rows), byref(record), loss.data_ptr(), byref(out), index, stream_of(index)))
     return loss, grad

@@ -84,15 +84,17 @@ def per_row(value: torch.Tensor, name: str, like: torch.Tensor, dtypes: tuple[to
     return value if value.is_contiguous() else value.contiguous()
 
 
-def device_of(tensor: torch.Tensor) -> torch.device:
-    """The CUDA device of ``tensor``; there is no other path."""
+def device_of(tensor: torch.Tensor) -> int:
+    """The index of the CUDA device of ``tensor``; there is no other path."""
     if not tensor.is_cuda:
         raise ValueError(f"logits must be on a CUDA device, not {tensor.device}")
-    return tensor.device
+    return tensor.get_device()
 
 
-def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def stream_of(index: int) -> int:
+    """The current stream of a CUDA device, as an address (``torch.cuda.current_stream`` without the Stream object,
+    which takes 2 us: these calls are as short as 10)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def top_logprobs(logits: torch.Tensor, k: int, *, temperature: float = 1.0) -> TopLogprobs:
@@ -108,12 +110,11 @@ def top_logprobs(logits: torch.Tensor, k: int, *, temperature: float = 1.0) -> T
         raise ValueError(f"k is {k}: 1 to {min(rows.vocab, _lib.WS_TOP_MAX_K)} are possible")
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError(f"temperature must be from 1e-6 to 1e6, not {temperature}")
-    device = device_of(logits)
+    index = device_of(logits)
     shape = (*logits.shape[:-1], k)
-    ids = torch.empty(shape, dtype=torch.int64, device=device)
-    logprobs = torch.empty(shape, dtype=torch.float32, device=device)
-    _lib.check(_lib.load().ws_top_logprobs(byref(rows), k, temperature, ids.data_ptr(), logprobs.data_ptr(), device.index,
-                                           stream_of(device)))
+    ids = logits.new_empty(shape, dtype=torch.int64)
+    logprobs = logits.new_empty(shape, dtype=torch.float32)
+    _lib.check(_lib.load().ws_top_logprobs(byref(rows), k, temperature, ids.data_ptr(), logprobs.data_ptr(), index, stream_of(index)))
     return TopLogprobs(ids, logprobs)
 
 
@@ -155,11 +156,11 @@ def sample(
     wide = isinstance(top_k, torch.Tensor) and top_k.dtype == torch.int64
     top_k_each, top_k = each(top_k, "top_k", (torch.int32, torch.int64))
     top_k = min(max(top_k, 0), _lib.WS_MAX_VOCAB)
-    device = device_of(logits)
+    index = device_of(logits)
     settings = _lib.Sampling(temperature_each, top_p_each, min_p_each, top_k_each, top_k, temperature, top_p, min_p, wide)
     shape = logits.shape[:-1]
-    tokens = torch.empty(shape, dtype=torch.int64, device=device)
-    logprobs = torch.empty(shape, dtype=torch.float32, device=device)
+    tokens = logits.new_empty(shape, dtype=torch.int64)
+    logprobs = logits.new_empty(shape, dtype=torch.float32)
     _lib.check(_lib.load().ws_sample(byref(rows), uniform.data_ptr(), byref(settings), tokens.data_ptr(), logprobs.data_ptr(),
-                                     device.index, stream_of(device)))
+                                     index, stream_of(index)))
     return Sampled(tokens, logprobs)
