@@ -12,35 +12,34 @@ namespace cg = cooperative_groups;
 
 // ------------------------------------------------------------ top log-probabilities
 //
-// One pass over the row gives its maximum m and S = sum exp((x - m) / t), and keeps
-// the candidates for the k largest logits in shared memory: a candidate is 64 bits, the order key
-// of its logit above the complement of its id, so that no two are equal and the
-// larger one comes first in the record.
+// One pass over the row gives its maximum m and S = sum exp((x - m) / t), and keeps in shared memory the
+// maximum of every thread's logits in every group of steps, 16 bits of its order key (up to kGroups
+// groups: one step each for a row of 2^17 16-bit logits). The k-th largest of the threads' maxima over the whole
+// row (for records of more than kFewMaxima, of four parts of it) is a lower bound of the k-th
+// largest logit, and a close one: about 1.15 k logits of a row reach it. So the pass itself costs a logit a share of one
+// comparison, and behind it the few groups whose maximum reaches the bound are read once more, out of
+// L2, for the logits that do.
 //
-// What a logit costs is one comparison of its unit's maximum with a threshold, below which nothing can be in
-// the record. The threshold comes from maxima that are at hand anyway: every thread keeps the maximum of what it
-// has seen (for records of more than kFewMaxima, one for each of its kUnits places in a step), which is
-// kRowThreads or more logits of different ids, and the k-th largest of those is a lower bound of the k-th
-// largest logit, and a close one. It is found by bisection over the upper 16 bits of the order keys after steps
-// 1, 4, 16, 64 and at the end; meanwhile a step adds about k candidates divided by the steps before the last
-// threshold.
-//
-// The list has room for k candidates and all of a step's that one unit of each thread
-// gives. A step that would overflow it (ascending or equal logits) is taken again unit
+// A candidate is 64 bits, the order key of its logit above the complement of its id, so that no two are equal and the
+// larger one comes first in the record. The list has room for k candidates and all that one unit of each thread
+// gives. A row of which more logits reach the bound (ascending or equal ones) is taken again unit
 // by unit, dropping all but the k largest before each: slow, and right for any row.
 constexpr uint32_t kTopDepth = 2;    // steps in flight
+constexpr uint32_t kGroups = 16;
 constexpr uint32_t kFewMaxima = 64;
 constexpr uint32_t kCandidates = WS_TOP_MAX_K + kRowThreads * 8;
 constexpr uint32_t kSorted = 512;  // candidates that are put in order by counting
 
 struct TopShared {
-  uint64_t list[kCandidates];
   uint64_t sorted[WS_TOP_MAX_K];  // the block's k largest in order
-  uint32_t count, sorted_count;
+  uint16_t maxima[kGroups][kRowThreads];
+  uint32_t bins[kRowThreads];
+  uint2 keys[kRowWarps], votes[2][kRowWarps];
   uint32_t sums[kRowWarps];
-  uint2 votes[2][kRowWarps];
   float2 soft[kRowWarps];
+  uint32_t count, sorted_count, bin, key;
 };
+static_assert(kCandidates * sizeof(uint64_t) <= kTopDepth * kStepBytes, "the list takes the ring's place");
 
 // What the blocks of a cluster tell each other of their shares of a row.
 struct TopTold {
@@ -52,48 +51,24 @@ struct TopTold {
 __device__ __forceinline__ uint64_t candidate(float x, uint32_t id) { return ((uint64_t)order_key(x) << 32) | (0xFFFFFFFFu - id); }
 __device__ __forceinline__ float candidate_value(uint64_t v) { return key_value((uint32_t)(v >> 32)); }
 
-// Keeps the k largest of s.list's first n > k candidates (in no order) and returns the smallest of these.
-__device__ __noinline__ uint64_t keep_largest(TopShared& s, uint32_t n, uint32_t k) {
+// Keeps the k largest of the first n > k candidates (in no order) and returns the smallest of these.
+__device__ __noinline__ uint64_t keep_largest(TopShared& s, uint64_t* list, uint32_t n, uint32_t k) {
   constexpr uint32_t kMine = (kCandidates + kRowThreads - 1) / kRowThreads;
   uint64_t mine[kMine];
 #pragma unroll
   for (uint32_t i = 0; i < kMine; ++i) {
     const uint32_t at = i * kRowThreads + threadIdx.x;
-    mine[i] = at < n ? s.list[at] : 0;
+    mine[i] = at < n ? list[at] : 0;
   }
+  // The k-th largest by bisection, two bits a round: how many reach each of three trials.
   uint64_t edge = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t trial = edge | (1ull << bit);
-    uint32_t c = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) c += mine[i] >= trial;
-    if (block_sum(c, s.sums) >= k) edge = trial;
-  }
-  if (threadIdx.x == 0) s.count = 0;
-  __syncthreads();
-#pragma unroll
-  for (uint32_t i = 0; i < kMine; ++i)
-    if (mine[i] >= edge) s.list[atomicAdd(&s.count, 1u)] = mine[i];
-  __syncthreads();
-  return edge;
-}
-
-// A logit that at least k of the block's maxima reach, as large as 16 bits of its order key
-// tell; the lowest finite number where fewer than k are above -inf. Two bits a round: the
-// counts of three trials by one reduction in the warp and one barrier.
-template <uint32_t N>
-__device__ __forceinline__ float kth_of_maxima(TopShared& s, const float (&top)[N], uint32_t k) {
-  uint32_t key[N];
-#pragma unroll
-  for (uint32_t j = 0; j < N; ++j) key[j] = order_key(top[j]) >> 16;
-  uint32_t edge = 0;
 #pragma unroll 1
-  for (int bit = 14; bit >= 0; bit -= 2) {
-    uint32_t low = 0, high = 0;  // counts of trials 1 and 2, and of trial 3
+  for (int bit = 62; bit >= 0; bit -= 2) {
+    uint32_t low = 0, high = 0;  // trials 1 and 2, and trial 3
 #pragma unroll
-    for (uint32_t j = 0; j < N; ++j) {
-      low += (key[j] >= (edge | (1u << bit)) ? 1u : 0u) + (key[j] >= (edge | (2u << bit)) ? 0x10000u : 0u);
-      high += key[j] >= (edge | (3u << bit)) ? 1u : 0u;
+    for (uint32_t i = 0; i < kMine; ++i) {
+      low += (mine[i] >= (edge | (1ull << bit)) ? 1u : 0u) + (mine[i] >= (edge | (2ull << bit)) ? 0x10000u : 0u);
+      high += mine[i] >= (edge | (3ull << bit)) ? 1u : 0u;
     }
     low = __reduce_add_sync(0xFFFFFFFFu, low);
     high = __reduce_add_sync(0xFFFFFFFFu, high);
@@ -106,145 +81,220 @@ __device__ __forceinline__ float kth_of_maxima(TopShared& s, const float (&top)[
       low += votes[w].x;
       high += votes[w].y;
     }
-    const uint32_t step = high >= k ? 3u : (low >> 16) >= k ? 2u : (low & 0xFFFFu) >= k ? 1u : 0u;
+    const uint64_t step = high >= k ? 3u : (low >> 16) >= k ? 2u : (low & 0xFFFFu) >= k ? 1u : 0u;
     edge |= step << bit;
   }
-  constexpr uint32_t kNone = 0x007Fu;  // upper half of -inf's key
-  return edge <= kNone ? -FLT_MAX : key_value(edge << 16);
-}
-
-template <uint32_t N>
-__device__ __forceinline__ float kth_threshold(TopShared& s, const float (&most)[N], uint32_t k) {
-  if (k > kFewMaxima) return kth_of_maxima(s, most, k);
-  float one[1] = {most[0]};
-#pragma unroll
-  for (uint32_t j = 1; j < N; ++j) one[0] = fmaxf(one[0], most[j]);
-  return kth_of_maxima(s, one, k);
-}
-
-// The step that begins at unit u0 again, from the `before` candidates there were, unit by unit; returns the new threshold.
-template <class T>
-__device__ __noinline__ float top_overflow(TopShared& s, Batch<T> now, uint32_t u0, uint32_t before, uint32_t k, uint32_t head,
-                                           float edge) {
+  if (threadIdx.x == 0) s.count = 0;
   __syncthreads();
-  if (threadIdx.x == 0) s.count = before;
+#pragma unroll
+  for (uint32_t i = 0; i < kMine; ++i)
+    if (mine[i] >= edge) list[atomicAdd(&s.count, 1u)] = mine[i];
+  __syncthreads();
+  return edge;
+}
+
+// All of units [first, last) that reach `bound`, unit by unit, with the list cut down to the k largest before each.
+template <class T>
+__device__ __noinline__ void top_by_units(TopShared& s, uint64_t* list, const RowWalk<T> walk, uint32_t first, uint32_t last, uint32_t k,
+                                          float bound) {
+  __syncthreads();
+  if (threadIdx.x == 0) s.count = 0;
   __syncthreads();
   uint64_t least = 0;
-#pragma unroll
-  for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
-    if (s.count > k) least = keep_largest(s, s.count, k);
+  for (uint32_t u0 = first; u0 < last; u0 += kRowThreads) {
+    if (s.count > k) least = keep_largest(s, list, s.count, k);
     __syncthreads();
-    float f[kUnit<T>];
-    unpack<T>(now.raw[j], f);
-    const uint32_t id = Batch<T>::unit(u0, j) * kUnit<T> - head;
+    const uint32_t u = u0 + threadIdx.x;
+    if (u < last) {
+      float f[kUnit<T>];
+      walk.load(u, f);
 #pragma unroll
-    for (uint32_t i = 0; i < kUnit<T>; ++i) {
-      if (f[i] >= edge) {
-        const uint64_t v = candidate(f[i], id + i);
-        if (v > least) s.list[atomicAdd(&s.count, 1u)] = v;
-      }
-    }
-    __syncthreads();
-  }
-  if (s.count > k) least = keep_largest(s, s.count, k);
-  __syncthreads();
-  return fmaxf(edge, least ? candidate_value(least) : -FLT_MAX);
-}
-
-// The k largest logits of what the block has read so far.
-template <class T>
-struct TopCollector {
-  using B = Batch<T>;
-  TopShared& s;
-  uint32_t k, head, step = 1;
-  float edge = -FLT_MAX;  // logits below it are of no use; nor are -inf and NaN
-  float most[B::kUnits];
-
-  __device__ __forceinline__ TopCollector(TopShared& shared, uint32_t k_, uint32_t head_) : s(shared), k(k_), head(head_) {
-    if (threadIdx.x == 0) s.count = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < B::kUnits; ++j) most[j] = -INFINITY;
-    __syncthreads();
-  }
-
-  // The step that begins at unit u0; top: the maxima of the thread's units in it.
-  __device__ __forceinline__ void add(const B& now, const float (&top)[B::kUnits], uint32_t u0) {
-    float all = top[0];
-#pragma unroll
-    for (uint32_t j = 0; j < B::kUnits; ++j) {
-      most[j] = fmaxf(most[j], top[j]);
-      all = fmaxf(all, top[j]);
-    }
-    // Steps 1, 4, 16, 64, ...: powers of 4.
-    if ((step & (step - 1)) == 0 && (step & 0x55555555u)) edge = fmaxf(edge, kth_threshold(s, most, k));
-    ++step;
-    const uint32_t before = s.count;
-    __syncthreads();  // everyone has it
-    if (all >= edge) {
-#pragma unroll
-      for (uint32_t j = 0; j < B::kUnits; ++j) {
-        if (top[j] >= edge) {
-          float f[kUnit<T>];
-          unpack<T>(now.raw[j], f);
-          const uint32_t id = B::unit(u0, j) * kUnit<T> - head;
-#pragma unroll
-          for (uint32_t i = 0; i < kUnit<T>; ++i) {
-            if (f[i] >= edge) {
-              const uint32_t at = atomicAdd(&s.count, 1u);
-              if (at < kCandidates) s.list[at] = candidate(f[i], id + i);
-            }
-          }
+      for (uint32_t i = 0; i < kUnit<T>; ++i) {
+        if (f[i] >= bound) {
+          const uint64_t v = candidate(f[i], u * kUnit<T> + i - walk.head);
+          if (v > least) list[atomicAdd(&s.count, 1u)] = v;
         }
       }
     }
     __syncthreads();
-    if (s.count > kCandidates) edge = top_overflow<T>(s, now, u0, before, k, head, edge);
   }
+}
 
-  // s.sorted_count (at most k) candidates in s.sorted, in order; visible behind the next barrier.
-  __device__ __forceinline__ void finish() {
-    edge = fmaxf(edge, kth_threshold(s, most, k));
-    constexpr uint32_t kMine = (kCandidates + kRowThreads - 1) / kRowThreads;
-    const uint32_t found = s.count;
-    uint64_t mine[kMine];
+// A logit that at least k of the block's maxima (N of each thread) reach, close to the k-th largest of them; the lowest finite
+// number where fewer than k are above -inf. The maxima are counted into bins between the largest and the smallest; the bound is the
+// smallest of those in the bins that hold the first k, which holds whatever the bins are.
+template <uint32_t N>
+__device__ __forceinline__ float kth_of_maxima(TopShared& s, const float (&most)[N], uint32_t k) {
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+  uint32_t key[N], hi = 0, lo = ~0u;
 #pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) {
-      const uint32_t at = i * kRowThreads + threadIdx.x;
-      mine[i] = at < found ? s.list[at] : 0;
+  for (uint32_t j = 0; j < N; ++j) {
+    key[j] = most[j] > -INFINITY ? order_key(most[j]) : 0;  // 0: none
+    hi = max(hi, key[j]);
+    lo = min(lo, key[j] ? key[j] : ~0u);
+  }
+  hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+  lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+  if (lane == 0) s.keys[warp] = make_uint2(hi, lo);
+  s.bins[threadIdx.x] = 0;
+  if (threadIdx.x == 0) s.key = ~0u;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t w = 0; w < kRowWarps; ++w) {
+    hi = max(hi, s.keys[w].x);
+    lo = min(lo, s.keys[w].y);
+  }
+  const float m = key_value(hi), scale = (float)(kRowThreads - 1) / fmaxf(m - key_value(lo), 1e-30f);
+  uint32_t bin[N];
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j) {
+    bin[j] = key[j] ? (uint32_t)fmaxf(fminf((m - most[j]) * scale, (float)(kRowThreads - 1)), 0.f) : ~0u;
+    if (key[j]) atomicAdd(&s.bins[bin[j]], 1u);
+  }
+  __syncthreads();
+  const uint32_t own = s.bins[threadIdx.x];
+  uint32_t all;
+  const uint32_t before = block_scan(own, s.sums, &all);
+  if (all < k) return -FLT_MAX;  // the same for the whole block
+  if (before < k && before + own >= k) s.bin = threadIdx.x;
+  __syncthreads();
+  const uint32_t last = s.bin;
+  uint32_t least = ~0u;
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j)
+    if (key[j] && bin[j] <= last) least = min(least, key[j]);
+  least = __reduce_min_sync(0xFFFFFFFFu, least);
+  if (lane == 0) atomicMin(&s.key, least);
+  __syncthreads();
+  return fmaxf(key_value(s.key), -FLT_MAX);
+}
+
+// The k largest logits of the units [first, last) that a block reads step by step. Where these are few (kGroups units a thread
+// or fewer), the groups are the units themselves.
+template <class T>
+struct TopCollector {
+  using B = Batch<T>;
+  TopShared& s;
+  uint32_t k, each, left, group = 0;  // steps a group has (0: it is a unit), and is still to get
+  float here = -INFINITY, most[B::kUnits];
+
+  __device__ __forceinline__ TopCollector(TopShared& shared, uint32_t k_, uint32_t first, uint32_t last) : s(shared), k(k_) {
+    const uint32_t steps = (last - first + B::kSpan - 1) / B::kSpan;
+    each = left = steps * B::kUnits <= kGroups ? 0 : (steps + kGroups - 1) / kGroups;
+#pragma unroll
+    for (uint32_t j = 0; j < B::kUnits; ++j) most[j] = -INFINITY;
+  }
+  // The next step, by the largest of the thread's logits in each unit and in all of them.
+  __device__ __forceinline__ void add(const float (&top)[B::kUnits], float all) {
+    if (each == 0) {
+#pragma unroll
+      for (uint32_t j = 0; j < B::kUnits; ++j) {
+        most[j] = fmaxf(most[j], top[j]);
+        put(top[j]);
+      }
+    } else {
+      here = fmaxf(here, all);
+      if (--left == 0) close();
+    }
+  }
+  // Behind the last step: s.sorted_count (at most k) candidates in s.sorted, in order; visible behind the next barrier. `list`:
+  // room for kCandidates that the ring has left.
+  __device__ __forceinline__ void finish(uint64_t* list, const RowWalk<T>& walk, uint32_t first, uint32_t last) {
+    if (left != each) close();
+    if (threadIdx.x == 0) s.count = 0;
+    float bound;
+    if (k > kFewMaxima) {
+      bound = kth_of_maxima(s, most, k);
+    } else {
+      const float one[1] = {fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))};
+      bound = kth_of_maxima(s, one, k);
+    }
+    const uint16_t key = (uint16_t)(order_key(bound) >> 16);
+    uint32_t hits = 0;
+    for (uint32_t g = 0; g < group; ++g) hits |= (s.maxima[g][threadIdx.x] >= key ? 1u : 0u) << g;
+    __syncthreads();  // every thread is done with the ring
+    while (hits) {
+      const uint32_t g = __ffs(hits) - 1;
+      hits &= hits - 1;
+      if (each == 0) {
+        const uint32_t u = B::unit(first + g / B::kUnits * B::kSpan, g % B::kUnits);
+        float f[kUnit<T>];
+        if (u < last) {
+          walk.load(u, f);
+          take(list, f, u * kUnit<T> - walk.head, bound);
+        }
+      }
+      for (uint32_t q = 0; q < each; ++q) {
+        const uint32_t u0 = first + (g * each + q) * B::kSpan;
+        float f[B::kUnits][kUnit<T>];
+#pragma unroll
+        for (uint32_t j = 0; j < B::kUnits; ++j)
+          if (B::unit(u0, j) < last) walk.load(B::unit(u0, j), f[j]);
+#pragma unroll
+        for (uint32_t j = 0; j < B::kUnits; ++j)
+          if (B::unit(u0, j) < last) take(list, f[j], B::unit(u0, j) * kUnit<T> - walk.head, bound);
+      }
     }
     __syncthreads();
-    if (threadIdx.x == 0) s.count = 0;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i)
-      if (mine[i] && candidate_value(mine[i]) >= edge) s.list[atomicAdd(&s.count, 1u)] = mine[i];
-    __syncthreads();
-    if (s.count > kSorted) keep_largest(s, s.count, k);  // k <= WS_TOP_MAX_K <= kSorted remain
+    if (s.count > kCandidates) top_by_units<T>(s, list, walk, first, last, k, bound);
+    if (s.count > kSorted) keep_largest(s, list, s.count, k);  // k <= WS_TOP_MAX_K <= kSorted remain
     const uint32_t n = s.count;
     if (threadIdx.x == 0) s.sorted_count = min(n, k);
+    // A candidate's place is the number of larger ones. The list is read eight at a time, up to 0s behind its end.
+    if (threadIdx.x < 8) list[n + threadIdx.x] = 0;
+    __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) {
-      const uint64_t v = s.list[i];
+      const uint64_t v = list[i];
       uint32_t place = 0;
-#pragma unroll 4
-      for (uint32_t q = 0; q < n; ++q) place += s.list[q] > v;
+      for (uint32_t q = 0; q < n; q += 8) {
+        ulonglong2 o[4];
+#pragma unroll
+        for (uint32_t h = 0; h < 4; ++h) o[h] = reinterpret_cast<const ulonglong2*>(list + q)[h];
+#pragma unroll
+        for (uint32_t h = 0; h < 4; ++h) place += (o[h].x > v) + (o[h].y > v);
+      }
       if (place < k) s.sorted[place] = v;
+    }
+  }
+
+ private:
+  __device__ __forceinline__ void put(float top) { s.maxima[group++][threadIdx.x] = (uint16_t)(order_key(top) >> 16); }
+  __device__ __forceinline__ void close() {
+#pragma unroll
+    for (uint32_t j = 0; j < B::kUnits; ++j)
+      if (group % B::kUnits == j) most[j] = fmaxf(most[j], here);
+    put(here);
+    here = -INFINITY;
+    left = each;
+  }
+  __device__ __forceinline__ void take(uint64_t* list, const float (&f)[kUnit<T>], uint32_t id, float bound) const {
+#pragma unroll
+    for (uint32_t i = 0; i < kUnit<T>; ++i) {
+      if (f[i] >= bound) {
+        const uint32_t at = atomicAdd(&s.count, 1u);
+        if (at < kCandidates) list[at] = candidate(f[i], id + i);
+      }
     }
   }
 };
 
-// The place of this block's i-th candidate in the cluster's record: i and how many of the other blocks' are larger.
-__device__ __forceinline__ uint32_t cluster_place(const RowCluster& cluster, const TopTold& told, uint32_t i, uint64_t v) {
-  uint32_t place = i;
-  for (uint32_t b = 0; b < cluster.blocks; ++b) {
-    if (b == cluster.rank) continue;
-    uint32_t lo = 0, hi = told.counts[b];
-    while (lo < hi) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (told.lists[b][mid] > v) lo = mid + 1;
-      else hi = mid;
-    }
-    place += lo;
+// The place of this block's i-th candidate in the cluster's record: i and how many of the other blocks' are larger. The
+// lists are searched side by side.
+__device__ __forceinline__ uint32_t cluster_place(const RowCluster& cluster, const TopTold& told, uint32_t k, uint32_t i, uint64_t v) {
+  uint32_t at[RowCluster::kMost], n[RowCluster::kMost];
+#pragma unroll
+  for (uint32_t b = 0; b < RowCluster::kMost; ++b) {
+    at[b] = 0;
+    n[b] = b < cluster.blocks && b != cluster.rank ? told.counts[b] : 0;
   }
+  for (uint32_t step = 1u << (31 - __clz(k)); step; step >>= 1) {
+#pragma unroll
+    for (uint32_t b = 0; b < RowCluster::kMost; ++b)
+      if (at[b] + step <= n[b] && told.lists[b][at[b] + step - 1] > v) at[b] += step;
+  }
+  uint32_t place = i;
+#pragma unroll
+  for (uint32_t b = 0; b < RowCluster::kMost; ++b) place += at[b];
   return place;
 }
 
@@ -252,6 +302,10 @@ __device__ __forceinline__ uint32_t cluster_place(const RowCluster& cluster, con
 __device__ __forceinline__ void tell_top(const RowCluster& cluster, const TopShared& s, TopTold* told) {
   const uint32_t n = s.sorted_count;
   for (uint32_t b = 0; b < cluster.blocks; ++b) {
+    if (b == cluster.rank) {
+      if (threadIdx.x == 0) told->counts[b] = n;
+      continue;
+    }
     TopTold* to = cluster.of(told, b);
     if (threadIdx.x < n) to->lists[cluster.rank][threadIdx.x] = s.sorted[threadIdx.x];
     if (threadIdx.x == 0) to->counts[cluster.rank] = n;
@@ -271,7 +325,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   uint32_t first, last;
   split_units(walk.units, cluster.rank, cluster.blocks, first, last);
   Ring<T, kTopDepth> ring(memory, walk, first, last);
-  TopCollector<T> top(s, k, walk.head);
+  TopCollector<T> top(s, k, first, last);
   Soft soft;
   for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
     Batch<T> b;
@@ -283,10 +337,10 @@ __global__ void __launch_bounds__(kRowThreads, 3)
       all = fmaxf(all, most[j]);
     }
     soft.add(b, all, c);
-    top.add(b, most, u0);
+    top.add(most, all);
     ring.advance();
   }
-  top.finish();
+  top.finish(reinterpret_cast<uint64_t*>(memory), walk, first, last);
   soft = block_soft(soft, c, s.soft);  // a barrier behind s.sorted, too
   uint32_t n = s.sorted_count;
   TopTold* told = reinterpret_cast<TopTold*>(memory + kTopDepth * kStepBytes);
@@ -303,7 +357,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   const size_t out = (size_t)row * k;
   if (threadIdx.x < s.sorted_count) {
     const uint64_t v = s.sorted[threadIdx.x];
-    const uint32_t place = cluster.blocks > 1 ? cluster_place(cluster, *told, threadIdx.x, v) : threadIdx.x;
+    const uint32_t place = cluster.blocks > 1 ? cluster_place(cluster, *told, k, threadIdx.x, v) : threadIdx.x;
     if (place < k) {
       ids[out + place] = (int64_t)(0xFFFFFFFFu - (uint32_t)v);
       logprobs[out + place] = (float)(((double)candidate_value(v) - (double)soft.m) * (double)inv_t - log_s);
@@ -322,8 +376,8 @@ __global__ void __launch_bounds__(kRowThreads, 3)
 // The tokens that top-k, top-p and min-p keep are a prefix of the row's order, so they are named by the
 // smallest logit kept and by how many of the tokens with that very logit are kept (those
 // with the lowest ids). Weights are 2^42 exp((x - m) / t) rounded to integers: 2^20 of
-// them fit 64 bits, sums are exact whatever their order, and what rounding and the 64-bit
-// exponential leave off is below 2^-42 of the largest weight a token.
+// them fit 64 bits, sums are exact whatever their order, and what rounding leaves off is 2^-43 of the
+// largest weight a token.
 //
 // One pass over the row gives (m, s) of every chunk (a warp's share of a step), in fp32, and, where tokens
 // are to be dropped, the largest logits as for a record. Most rows are decided by these:
@@ -363,6 +417,7 @@ struct SampleShared {
   double sums[kRowWarps];
   unsigned long long weight[WS_TOP_MAX_K];
   uint64_t merged[WS_TOP_MAX_K];  // the row's largest, in order, where it has several blocks
+  double roots[16];
   double chunk_before;
   uint32_t chunk;
   uint32_t key_lo, key_hi;
@@ -380,7 +435,7 @@ __device__ __forceinline__ int64_t top_k_of(const ws_sampling& p, uint32_t row) 
 struct SampleSettings {
   float t, top_p, min_p;
   int64_t top_k;
-  double u;
+  double u, log_min_p;
 
   __device__ __forceinline__ SampleSettings(const ws_sampling& p, const float* uniform, uint32_t row) {
     t = p.temperature_each ? p.temperature_each[row] : p.temperature;
@@ -388,6 +443,7 @@ struct SampleSettings {
     min_p = fminf(p.min_p_each ? p.min_p_each[row] : p.min_p, 1.f);
     top_k = top_k_of(p, row);
     u = (double)uniform[row];
+    log_min_p = min_p > 0.f ? log2((double)min_p) : -INFINITY;
     if (!(t > 0.f)) {
       t = 1.f;
       top_k = 1;
@@ -408,18 +464,35 @@ struct SampleRow {
   RowWalk<T> walk;
   uint32_t first, last;
   float m;
-  double inv_t;
+  double inv_t, log2_t;  // 1 and log2(e) over the temperature
+  const double* roots;   // 2^(i / 16) for i from 0 to 15
 
-  __device__ __forceinline__ double weight(float v) const { return v == m ? 1.0 : exp(((double)v - (double)m) * inv_t); }
-  __device__ __forceinline__ unsigned long long fixed(float v) const {
-    return v == m ? (unsigned long long)kWeightOne : __double2ull_rn(weight(v) * kWeightOne);
+  // log2 of a token's weight.
+  __device__ __forceinline__ double log_weight(float v) const { return v == m ? 0.0 : ((double)v - (double)m) * log2_t; }
+  // 2^(y + 42) rounded to an integer, y <= 0. With n / 16 next to y, 2^y = 2^(n / 16) 2^f with |f| <= 1/32, and 2^f
+  // is e^(f ln 2) by its series up to the 6th power, off by 5e-16. Adding 2^10 leaves the multiple of 2^-42 in the sum's lower bits.
+  __device__ __forceinline__ unsigned long long fixed(double y) const {
+    if (!(y > -44.0)) return 0;
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: behind it a sum has no fraction
+    const double k = fma(y, 16.0, kRound);
+    const int n = __double2loint(k);
+    const double g = fma(k - kRound, -1.0 / 16, y) * 0.693147180559945309417;
+    double p = 1.0 / 720;
+    p = fma(p, g, 1.0 / 120);
+    p = fma(p, g, 1.0 / 24);
+    p = fma(p, g, 1.0 / 6);
+    p = fma(p, g, 0.5);
+    p = fma(p, g, 1.0);
+    p = fma(p, g, 1.0) * roots[n & 15];
+    p = __hiloint2double(__double2hiint(p) + (n >> 4) * (1 << 20), __double2loint(p)) + 1024.0;
+    return (unsigned long long)(__double_as_longlong(p) - __double_as_longlong(1024.0));
   }
   // As it counts when the token is drawn.
   __device__ __forceinline__ unsigned long long kept(float v, const SampleSettings& p) const {
-    const double w = weight(v);
-    if (p.min_p > 0.f && !(w >= (double)p.min_p)) return 0;
-    const unsigned long long f = __double2ull_rn(w * kWeightOne);
-    return p.first() && f == 0 && w > 0.0 ? 1 : f;
+    const double y = log_weight(v);
+    if (!(y >= p.log_min_p)) return 0;
+    const unsigned long long w = fixed(y);
+    return p.first() && w == 0 && y > -1075.0 ? 1 : w;
   }
   // visit(logit) for every logit of the block's part above -inf.
   template <class F>
@@ -501,7 +574,7 @@ __device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, b
   row.each([&](float v) {
     const int d = digit(v);
     if (d < 0) return;
-    const unsigned long long w = weigh ? row.fixed(v) : 0;
+    const unsigned long long w = weigh ? row.fixed(row.log_weight(v)) : 0;
     if (d == (int)kBins - 1) {
       ++tail_count;
       tail_mass += w;
@@ -606,7 +679,7 @@ __device__ Kept find_edge(SampleShared& s, Bins& bins, const SampleRow<T>& row, 
   }
   Kept kept;
   kept.edge = key_value(prefix);
-  const unsigned long long one = row.fixed(kept.edge);
+  const unsigned long long one = row.fixed(row.log_weight(kept.edge));
   kept.ties = weigh ? (uint32_t)min((unsigned long long)at, (target + one - 1) / max(one, 1ull)) : (uint32_t)target;
   return kept;
 }
@@ -628,9 +701,9 @@ __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const Sa
   }
   if (p.top_p < 1.f && p.top_k != 1) {
     unsigned long long above = 0;
-    row.each([&](float v) { above += v > kept.edge ? row.fixed(v) : 0; });
+    row.each([&](float v) { above += v > kept.edge ? row.fixed(row.log_weight(v)) : 0; });
     above = cluster_sum(above, s);
-    const unsigned long long one = kept.edge > -INFINITY ? row.fixed(kept.edge) : 0;
+    const unsigned long long one = kept.edge > -INFINITY ? row.fixed(row.log_weight(kept.edge)) : 0;
     const unsigned long long total = above + one * kept.ties;
     unsigned long long target = (unsigned long long)ceil((double)p.top_p * (double)total);
     target = min(max(target, 1ull), total);
@@ -738,8 +811,8 @@ __device__ __forceinline__ bool token_of_largest(SampleShared& s, const SampleRo
   bool whole = all_there || (limited && p.top_k <= (int64_t)n);  // the list holds all that top-k keeps
   const uint32_t id = i < n ? 0xFFFFFFFFu - (uint32_t)list[i] : 0xFFFFFFFFu;
   const float v = i < n ? candidate_value(list[i]) : -INFINITY;
-  const double weight = i < n ? row.weight(v) : 0.0;
-  const unsigned long long fixed = __double2ull_rn(weight * kWeightOne);
+  const double y = i < n ? row.log_weight(v) : -INFINITY;
+  const unsigned long long fixed = row.fixed(y);
   uint32_t keep = n;
   if (p.top_p < 1.f && p.top_k != 1) {
     unsigned long long sum;
@@ -759,12 +832,12 @@ __device__ __forceinline__ bool token_of_largest(SampleShared& s, const SampleRo
     }
   }
   if (p.min_p > 0.f) {
-    const uint32_t heavy = __syncthreads_count(i < keep && weight >= (double)p.min_p);
+    const uint32_t heavy = __syncthreads_count(i < keep && y >= p.log_min_p);
     whole = whole || heavy < keep;
     keep = heavy;
   }
   if (!whole) return false;
-  const unsigned long long w = i < keep ? (p.first() && fixed == 0 && weight > 0.0 ? 1 : fixed) : 0;
+  const unsigned long long w = i < keep ? (p.first() && fixed == 0 && y > -1075.0 ? 1 : fixed) : 0;
   const unsigned long long sum = block_sum(w, s.scan);
   const unsigned long long need = p.need(sum);
   s.weight[i] = w;
@@ -794,7 +867,8 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   const uint32_t chunks = (walk.units + kChunkUnits - 1) / kChunkUnits;
   uint32_t chunk0, chunk1;
   split_units(chunks, cluster.rank, cluster.blocks, chunk0, chunk1);
-  SampleRow<T> row{walk, chunk0 * kChunkUnits, min(chunk1 * kChunkUnits, walk.units), 0.f, 1.0 / (double)p.t};
+  SampleRow<T> row{walk, chunk0 * kChunkUnits, min(chunk1 * kChunkUnits, walk.units), 0.f, 1.0 / (double)p.t,
+                   1.442695040888963407360 / (double)p.t, s.roots};
   row.first = min(row.first, row.last);
   float2* soft = reinterpret_cast<float2*>(memory + kTopDepth * kStepBytes);
   TopTold* told = reinterpret_cast<TopTold*>(soft + ((chunks + 1) & ~1u));
@@ -803,8 +877,9 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   const uint32_t k = p.top_k >= 1 && p.top_k <= WS_TOP_MAX_K ? (uint32_t)p.top_k : WS_TOP_MAX_K;
 
   Ring<T, kTopDepth> ring(memory, walk, row.first, row.last);
-  TopCollector<T> top(s.top, k, walk.head);
+  TopCollector<T> top(s.top, k, row.first, row.last);
   if (threadIdx.x == 0) s.token = ~0ull;
+  if (threadIdx.x < 16) s.roots[threadIdx.x] = exp2(threadIdx.x / 16.0);
   for (uint32_t u0 = row.first; u0 < row.last; u0 += Batch<T>::kSpan) {
     Batch<T> b;
     ring.read(b);
@@ -820,10 +895,10 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     const uint32_t ch = u0 / kChunkUnits + warp;
     if (lane == 0 && ch < chunk1) soft[ch] = make_float2(m, sum);
-    if (dropping) top.add(b, most, u0);
+    if (dropping) top.add(most, all);
     ring.advance();
   }
-  if (dropping) top.finish();
+  if (dropping) top.finish(reinterpret_cast<uint64_t*>(memory), walk, row.first, row.last);
   __syncthreads();
   const uint64_t* list = s.top.sorted;
   uint32_t n = dropping ? s.top.sorted_count : 0;
@@ -842,7 +917,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       for (uint32_t b = 0; b < cluster.blocks; ++b) n += told->counts[b];
       if (threadIdx.x < own) {
         const uint64_t v = s.top.sorted[threadIdx.x];
-        const uint32_t place = cluster_place(cluster, *told, threadIdx.x, v);
+        const uint32_t place = cluster_place(cluster, *told, k, threadIdx.x, v);
         if (place < k)
           for (uint32_t b = 0; b < cluster.blocks; ++b) cluster.of(s.merged, b)[place] = v;
       }
