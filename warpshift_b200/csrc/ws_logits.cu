@@ -28,7 +28,8 @@ constexpr uint32_t kTopDepth = 2;    // steps in flight
 constexpr uint32_t kGroups = 16;
 constexpr uint32_t kFewMaxima = 64;
 constexpr uint32_t kCandidates = WS_TOP_MAX_K + kRowThreads * 8;
-constexpr uint32_t kSorted = 512;  // candidates that are put in order by counting
+constexpr uint32_t kCounted = 128;  // candidates that are put in order by counting
+constexpr uint32_t kSorted = 512;   // and by sorting
 
 struct TopShared {
   uint64_t sorted[WS_TOP_MAX_K];  // the block's k largest in order
@@ -37,9 +38,10 @@ struct TopShared {
   uint2 keys[kRowWarps], votes[2][kRowWarps];
   uint32_t sums[kRowWarps];
   float2 soft[kRowWarps];
-  uint32_t count, sorted_count, bin, key;
+  uint32_t count, queued, sorted_count, bin, key;
 };
-static_assert(kCandidates * sizeof(uint64_t) <= kTopDepth * kStepBytes, "the list takes the ring's place");
+static_assert(kCandidates * sizeof(uint64_t) + kGroups * kRowThreads * sizeof(uint16_t) <= kTopDepth * kStepBytes,
+              "the list and the queue take the ring's place");
 
 // What the blocks of a cluster tell each other of their shares of a row.
 struct TopTold {
@@ -169,6 +171,45 @@ __device__ __forceinline__ float kth_of_maxima(TopShared& s, const float (&most)
   return fmaxf(key_value(s.key), -FLT_MAX);
 }
 
+// Up to kSorted candidates in descending order: the k largest into s.sorted. A bitonic network, two neighbours to a thread: exchanges
+// over up to 32 places stay within a warp. Counting larger ones instead takes n^2 comparisons: as fast at 128 candidates, 2.5 times as
+// long at 300.
+__device__ __noinline__ void sort_largest(TopShared& s, uint64_t* list, uint32_t n, uint32_t k) {
+  const uint32_t t = threadIdx.x, places = n <= kSorted / 2 ? kSorted / 2 : kSorted;
+  __syncthreads();
+  uint64_t a = 2 * t < n ? list[2 * t] : 0, b = 2 * t + 1 < n ? list[2 * t + 1] : 0;
+  for (uint32_t size = 2; size <= places; size *= 2) {
+    const bool down = (2 * t & size) == 0;
+    for (uint32_t far = size / 2; far; far /= 2) {
+      uint64_t oa, ob;
+      if (far == 1) {
+        if ((a < b) == down) {
+          const uint64_t c = a;
+          a = b;
+          b = c;
+        }
+        continue;
+      }
+      if (far <= 32) {
+        oa = __shfl_xor_sync(0xFFFFFFFFu, a, far / 2);
+        ob = __shfl_xor_sync(0xFFFFFFFFu, b, far / 2);
+      } else {
+        __syncthreads();
+        list[t] = a;
+        list[kRowThreads + t] = b;
+        __syncthreads();
+        oa = list[t ^ (far / 2)];
+        ob = list[kRowThreads + (t ^ (far / 2))];
+      }
+      const bool larger = ((2 * t & far) == 0) == down;
+      a = (a > oa) == larger ? a : oa;
+      b = (b > ob) == larger ? b : ob;
+    }
+  }
+  if (2 * t < k) s.sorted[2 * t] = a;
+  if (2 * t + 1 < k) s.sorted[2 * t + 1] = b;
+}
+
 // The k largest logits of the units [first, last) that a block reads step by step. Where these are few (kGroups units a thread
 // or fewer), the groups are the units themselves.
 template <class T>
@@ -201,7 +242,8 @@ struct TopCollector {
   // room for kCandidates that the ring has left.
   __device__ __forceinline__ void finish(uint64_t* list, const RowWalk<T>& walk, uint32_t first, uint32_t last) {
     if (left != each) close();
-    if (threadIdx.x == 0) s.count = 0;
+    if (threadIdx.x == 0) s.count = s.queued = 0;
+    uint16_t* queue = reinterpret_cast<uint16_t*>(list + kCandidates);
     float bound;
     if (k > kFewMaxima) {
       bound = kth_of_maxima(s, most, k);
@@ -210,29 +252,21 @@ struct TopCollector {
       bound = kth_of_maxima(s, one, k);
     }
     const uint16_t key = (uint16_t)(order_key(bound) >> 16);
-    uint32_t hits = 0;
-    for (uint32_t g = 0; g < group; ++g) hits |= (s.maxima[g][threadIdx.x] >= key ? 1u : 0u) << g;
+    // The groups that reach it, in a queue that all threads work off.
     __syncthreads();  // every thread is done with the ring
-    while (hits) {
-      const uint32_t g = __ffs(hits) - 1;
-      hits &= hits - 1;
-      if (each == 0) {
-        const uint32_t u = B::unit(first + g / B::kUnits * B::kSpan, g % B::kUnits);
+    for (uint32_t g = 0; g < group; ++g)
+      if (s.maxima[g][threadIdx.x] >= key) queue[atomicAdd(&s.queued, 1u)] = (uint16_t)(g * kRowThreads + threadIdx.x);
+    __syncthreads();
+    // Of a hit of several units, a thread takes one after the other.
+    const uint32_t parts = each ? each * B::kUnits : 1, work = s.queued * parts;
+    for (uint32_t i = threadIdx.x; i < work; i += kRowThreads) {
+      const uint32_t hit = queue[i / parts], part = i % parts, g = hit / kRowThreads, who = hit % kRowThreads;
+      const uint32_t step = each ? g * each + part / B::kUnits : g / B::kUnits, j = (each ? part : g) % B::kUnits;
+      const uint32_t u = first + step * B::kSpan + (who >> 5) * B::kWarpSpan + j * 32 + (who & 31u);
+      if (u < last) {
         float f[kUnit<T>];
-        if (u < last) {
-          walk.load(u, f);
-          take(list, f, u * kUnit<T> - walk.head, bound);
-        }
-      }
-      for (uint32_t q = 0; q < each; ++q) {
-        const uint32_t u0 = first + (g * each + q) * B::kSpan;
-        float f[B::kUnits][kUnit<T>];
-#pragma unroll
-        for (uint32_t j = 0; j < B::kUnits; ++j)
-          if (B::unit(u0, j) < last) walk.load(B::unit(u0, j), f[j]);
-#pragma unroll
-        for (uint32_t j = 0; j < B::kUnits; ++j)
-          if (B::unit(u0, j) < last) take(list, f[j], B::unit(u0, j) * kUnit<T> - walk.head, bound);
+        walk.load(u, f);
+        take(list, f, u * kUnit<T> - walk.head, bound);
       }
     }
     __syncthreads();
@@ -240,11 +274,15 @@ struct TopCollector {
     if (s.count > kSorted) keep_largest(s, list, s.count, k);  // k <= WS_TOP_MAX_K <= kSorted remain
     const uint32_t n = s.count;
     if (threadIdx.x == 0) s.sorted_count = min(n, k);
+    if (n > kCounted) {
+      sort_largest(s, list, n, k);
+      return;
+    }
     // A candidate's place is the number of larger ones. The list is read eight at a time, up to 0s behind its end.
     if (threadIdx.x < 8) list[n + threadIdx.x] = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) {
-      const uint64_t v = list[i];
+    if (threadIdx.x < n) {
+      const uint64_t v = list[threadIdx.x];
       uint32_t place = 0;
       for (uint32_t q = 0; q < n; q += 8) {
         ulonglong2 o[4];
@@ -268,11 +306,16 @@ struct TopCollector {
     left = each;
   }
   __device__ __forceinline__ void take(uint64_t* list, const float (&f)[kUnit<T>], uint32_t id, float bound) const {
+    uint32_t mask = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kUnit<T>; ++i) mask |= (f[i] >= bound ? 1u : 0u) << i;
+    if (!mask) return;
+    uint32_t at = atomicAdd(&s.count, (uint32_t)__popc(mask));
 #pragma unroll
     for (uint32_t i = 0; i < kUnit<T>; ++i) {
-      if (f[i] >= bound) {
-        const uint32_t at = atomicAdd(&s.count, 1u);
+      if (mask >> i & 1u) {
         if (at < kCandidates) list[at] = candidate(f[i], id + i);
+        ++at;
       }
     }
   }
@@ -289,8 +332,11 @@ __device__ __forceinline__ uint32_t cluster_place(const RowCluster& cluster, con
   }
   for (uint32_t step = 1u << (31 - __clz(k)); step; step >>= 1) {
 #pragma unroll
-    for (uint32_t b = 0; b < RowCluster::kMost; ++b)
-      if (at[b] + step <= n[b] && told.lists[b][at[b] + step - 1] > v) at[b] += step;
+    for (uint32_t b = 0; b < RowCluster::kMost; ++b) {
+      const uint32_t next = at[b] + step;
+      const uint64_t o = told.lists[b][min(next, (uint32_t)WS_TOP_MAX_K) - 1];  // read in any case: the searches do not wait for one another
+      at[b] = next <= n[b] && o > v ? next : at[b];
+    }
   }
   uint32_t place = i;
 #pragma unroll
@@ -405,7 +451,12 @@ struct ChunkSums {
   unsigned long long mass[kChunks];
   uint32_t ties[kChunks];
 };
-static_assert(sizeof(Bins) <= kTopDepth * kStepBytes && sizeof(ChunkSums) <= kTopDepth * kStepBytes, "they take the ring's place");
+// What exact_token has in the ring's place: the tokens of the block's part that may be kept, once they are few, and the counts of a pass.
+struct ExactShared {
+  uint64_t list[kCandidates];
+  Bins bins;
+};
+static_assert(sizeof(ExactShared) <= kTopDepth * kStepBytes && sizeof(ChunkSums) <= kTopDepth * kStepBytes, "they take the ring's place");
 
 struct SampleShared {
   TopShared top;
@@ -494,15 +545,31 @@ struct SampleRow {
     const unsigned long long w = fixed(y);
     return p.first() && w == 0 && y > -1075.0 ? 1 : w;
   }
-  // visit(logit) for every logit of the block's part above -inf.
+  // visit(logit, id) for every logit of the block's part above -inf, or for those in `list`, where there is one. Four units a thread are
+  // on their way at once.
   template <class F>
-  __device__ __forceinline__ void each(F&& visit) const {
-    for (uint32_t u = first + threadIdx.x; u < last; u += kRowThreads) {
-      float f[kUnit<T>];
-      walk.load(u, f);
+  __device__ __forceinline__ void each(const uint64_t* list, uint32_t n, F&& visit) const {
+    if (list) {
+      for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) visit(candidate_value(list[i]), 0xFFFFFFFFu - (uint32_t)list[i]);
+      return;
+    }
+    for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
+      float f[Batch<T>::kUnits][kUnit<T>];
 #pragma unroll
-      for (uint32_t i = 0; i < kUnit<T>; ++i)
-        if (f[i] > -INFINITY) visit(f[i]);
+      for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+        const uint32_t u = Batch<T>::unit(u0, j);
+        if (u < last) {
+          walk.load(u, f[j]);
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < kUnit<T>; ++i) f[j][i] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < Batch<T>::kUnits; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < kUnit<T>; ++i)
+          if (f[j][i] > -INFINITY) visit(f[j][i], Batch<T>::unit(u0, j) * kUnit<T> + i - walk.head);
     }
   }
 };
@@ -558,11 +625,17 @@ __device__ __forceinline__ unsigned long long cluster_sum(unsigned long long v, 
   return t;
 }
 
+// The tokens that may still be kept, if they are in `list`; all of the block's part otherwise.
+struct Few {
+  const uint64_t* list = nullptr;
+  uint32_t n = 0;
+};
+
 // One counting pass: digit(logit) in [0, kBins) for those that take part, or -1; in every bin how many they are and, where
 // `weigh`, their weight. Finds the lowest digit at which the running total (of counts, or of weights where
 // `weigh`) reaches `target`: s.found_*. The last bin, which may take most of a row, is counted in registers.
 template <class T, class D>
-__device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, bool weigh, unsigned long long target, D&& digit) {
+__device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, const Few& few, bool weigh, unsigned long long target, D&& digit) {
   cg::cluster_group cluster = cg::this_cluster();
   for (uint32_t i = threadIdx.x; i < kBins; i += kRowThreads) {
     bins.count[i] = 0;
@@ -571,7 +644,7 @@ __device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, b
   __syncthreads();
   uint32_t tail_count = 0;
   unsigned long long tail_mass = 0;
-  row.each([&](float v) {
+  row.each(few.list, few.n, [&](float v, uint32_t) {
     const int d = digit(v);
     if (d < 0) return;
     const unsigned long long w = weigh ? row.fixed(row.log_weight(v)) : 0;
@@ -622,18 +695,33 @@ __device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, b
 // The logit at which the total over the row in descending order reaches `target` (1 <= target <= the
 // total), among logits above `floor`, and how many of the tokens with this very logit it takes.
 template <class T>
-__device__ Kept find_edge(SampleShared& s, Bins& bins, const SampleRow<T>& row, bool weigh, unsigned long long target, float floor) {
+__device__ Kept find_edge(SampleShared& s, ExactShared& m, const SampleRow<T>& row, Few& few, bool weigh, unsigned long long target, float floor) {
   cg::cluster_group cluster = cg::this_cluster();
+  Bins& bins = m.bins;
   // First by distance from the maximum, 1/64 of a temperature a bin and one for all that is 16 below.
   const float scale = fminf((float)(64.0 * row.inv_t), 3e38f);
   auto coarse = [&](float v) { return v == row.m ? 0 : (int)fminf((row.m - v) * scale, (float)(kBins - 1)); };
-  find_bin(s, bins, row, weigh, target, [&](float v) { return v > floor ? coarse(v) : -1; });
+  find_bin(s, bins, row, few, weigh, target, [&](float v) { return v > floor ? coarse(v) : -1; });
   const int bin = (int)s.found_bin;
   target -= s.found_before;
   uint32_t at = s.found_count;
+  // Nothing below this bin is kept: if what is above is few in this block, the passes to come need not go over the row.
+  if (!few.list) {
+    if (threadIdx.x == 0) s.top.count = 0;
+    __syncthreads();
+    row.each(nullptr, 0, [&](float v, uint32_t id) {
+      if (v > floor && coarse(v) <= bin) {
+        const uint32_t i = atomicAdd(&s.top.count, 1u);
+        if (i < kCandidates) m.list[i] = candidate(v, id);
+      }
+    });
+    __syncthreads();
+    // The edge lies above the floor, so that tokens at the floor itself are not kept. The list has the counts of up to kBins chunks beside it.
+    if (s.top.count <= kCandidates && row.last - row.first <= kBins * kChunkUnits) few = Few{m.list, s.top.count};
+  }
   // Then by the order keys of the bin's logits, from the first bit in which they differ.
   uint32_t lo = 0xFFFFFFFFu, hi = 0;
-  row.each([&](float v) {
+  row.each(few.list, few.n, [&](float v, uint32_t) {
     if (v > floor && coarse(v) == bin) {
       const uint32_t k = order_key(v);
       lo = min(lo, k);
@@ -665,7 +753,7 @@ __device__ Kept find_edge(SampleShared& s, Bins& bins, const SampleRow<T>& row, 
     const int step = min(left, 8);
     const int shift = left - step;
     // The largest digit first: digits are counted from the top.
-    find_bin(s, bins, row, weigh, target, [&](float v) {
+    find_bin(s, bins, row, few, weigh, target, [&](float v) {
       if (!(v > floor) || coarse(v) != bin) return -1;
       const uint32_t k = order_key(v);
       if (left < 32 && (k >> left) != prefix) return -1;
@@ -689,19 +777,20 @@ __device__ Kept find_edge(SampleShared& s, Bins& bins, const SampleRow<T>& row, 
 template <class T>
 __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const SampleRow<T>& row, const SampleSettings& p, uint32_t vocab) {
   cg::cluster_group cluster = cg::this_cluster();
-  Bins& bins = *reinterpret_cast<Bins*>(memory);
+  ExactShared& m = *reinterpret_cast<ExactShared*>(memory);
+  Few few;
   Kept kept;
   if (p.top_k == 1) {
     kept.edge = row.m;
     kept.ties = 1;
   } else if (p.top_k > 1 && p.top_k < (int64_t)vocab) {
     unsigned long long there = 0;
-    row.each([&](float) { ++there; });
-    if (cluster_sum(there, s) > (unsigned long long)p.top_k) kept = find_edge(s, bins, row, false, (unsigned long long)p.top_k, -INFINITY);
+    row.each(nullptr, 0, [&](float, uint32_t) { ++there; });
+    if (cluster_sum(there, s) > (unsigned long long)p.top_k) kept = find_edge(s, m, row, few, false, (unsigned long long)p.top_k, -INFINITY);
   }
   if (p.top_p < 1.f && p.top_k != 1) {
     unsigned long long above = 0;
-    row.each([&](float v) { above += v > kept.edge ? row.fixed(row.log_weight(v)) : 0; });
+    row.each(few.list, few.n, [&](float v, uint32_t) { above += v > kept.edge ? row.fixed(row.log_weight(v)) : 0; });
     above = cluster_sum(above, s);
     const unsigned long long one = kept.edge > -INFINITY ? row.fixed(row.log_weight(kept.edge)) : 0;
     const unsigned long long total = above + one * kept.ties;
@@ -710,39 +799,70 @@ __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const Sa
     if (target > above)
       kept.ties = min(kept.ties, (uint32_t)((target - above + one - 1) / max(one, 1ull)));
     else
-      kept = find_edge(s, bins, row, true, target, kept.edge);
+      kept = find_edge(s, m, row, few, true, target, kept.edge);
   }
 
   // Weights of the tokens kept, in id order: by chunks, then within the chunk that holds the token.
-  ChunkSums& sums = *reinterpret_cast<ChunkSums*>(memory);
+  // By chunk of the block's part; beside the list, where there is one (find_edge sees to it that they fit).
   const bool edged = kept.edge > -INFINITY;
   const unsigned long long one = edged ? row.kept(kept.edge, p) : 0;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const uint32_t chunk0 = row.first / kChunkUnits;
   const uint32_t chunk1 = row.first < row.last ? (row.last + kChunkUnits - 1) / kChunkUnits : chunk0;
+  unsigned long long* chunk_mass = few.list ? m.bins.mass : reinterpret_cast<ChunkSums*>(memory)->mass;
+  uint32_t* chunk_ties = few.list ? m.bins.count : reinterpret_cast<ChunkSums*>(memory)->ties;
   unsigned long long mass = 0;
   uint32_t tied = 0;
   __syncthreads();
-  for (uint32_t ch = chunk0 + warp; ch < chunk1; ch += kRowWarps) {
-    unsigned long long w = 0;
-    uint32_t e = 0;
-    for (uint32_t u = ch * kChunkUnits + lane; u < min((ch + 1) * kChunkUnits, row.last); u += 32) {
-      float f[kUnit<T>];
-      row.walk.load(u, f);
-#pragma unroll
-      for (uint32_t i = 0; i < kUnit<T>; ++i) {
-        if (f[i] > kept.edge) w += row.kept(f[i], p);
-        e += edged && f[i] == kept.edge;
-      }
+  if (few.list) {
+    for (uint32_t c = threadIdx.x; c < chunk1 - chunk0; c += kRowThreads) {
+      chunk_mass[c] = 0;
+      chunk_ties[c] = 0;
     }
+    __syncthreads();
+    row.each(few.list, few.n, [&](float v, uint32_t id) {
+      const uint32_t c = (id + row.walk.head) / kChunk<T> - chunk0;
+      if (v > kept.edge) {
+        const unsigned long long w = row.kept(v, p);
+        atomicAdd(&chunk_mass[c], w);
+        mass += w;
+      } else if (v == kept.edge) {
+        atomicAdd(&chunk_ties[c], 1u);
+        ++tied;
+      }
+    });
+  } else {
+    for (uint32_t ch = chunk0 + warp; ch < chunk1; ch += kRowWarps) {
+      unsigned long long w = 0;
+      uint32_t e = 0;
+      float f[Batch<T>::kUnits][kUnit<T>];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
-    e = __reduce_add_sync(0xFFFFFFFFu, e);
-    if (lane == 0) {
-      sums.mass[ch - chunk0] = w;
-      sums.ties[ch - chunk0] = e;
-      mass += w;
-      tied += e;
+      for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+        const uint32_t u = ch * kChunkUnits + j * 32 + lane;
+        if (u < row.last) {
+          row.walk.load(u, f[j]);
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < kUnit<T>; ++i) f[j][i] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+#pragma unroll
+        for (uint32_t i = 0; i < kUnit<T>; ++i) {
+          if (f[j][i] > kept.edge) w += row.kept(f[j][i], p);
+          e += edged && f[j][i] == kept.edge;
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+      e = __reduce_add_sync(0xFFFFFFFFu, e);
+      if (lane == 0) {
+        chunk_mass[ch - chunk0] = w;
+        chunk_ties[ch - chunk0] = e;
+        mass += w;
+        tied += e;
+      }
     }
   }
   mass = block_sum(mass, s.scan);
@@ -772,25 +892,25 @@ __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const Sa
     const uint32_t n = chunk1 - chunk0, each = (n + kRowThreads - 1) / kRowThreads;
     const uint32_t c0 = min(threadIdx.x * each, n), c1 = min(c0 + each, n);
     uint32_t e = 0, all_ties;
-    for (uint32_t c = c0; c < c1; ++c) e += sums.ties[c];
+    for (uint32_t c = c0; c < c1; ++c) e += chunk_ties[c];
     uint32_t tie = ties_before + block_scan(e, s.top.sums, &all_ties);
     const uint32_t tie0 = tie;
     unsigned long long w = 0, all;
     for (uint32_t c = c0; c < c1; ++c) {
-      w += sums.mass[c] + one * (min(tie + sums.ties[c], kept.ties) - min(tie, kept.ties));
-      tie += sums.ties[c];
+      w += chunk_mass[c] + one * (min(tie + chunk_ties[c], kept.ties) - min(tie, kept.ties));
+      tie += chunk_ties[c];
     }
     unsigned long long at = before + block_scan(w, s.scan, &all);
     tie = tie0;
     for (uint32_t c = c0; c < c1; ++c) {
-      const unsigned long long own = sums.mass[c] + one * (min(tie + sums.ties[c], kept.ties) - min(tie, kept.ties));
+      const unsigned long long own = chunk_mass[c] + one * (min(tie + chunk_ties[c], kept.ties) - min(tie, kept.ties));
       if (at < need && need <= at + own) {
         s.chunk = chunk0 + c;
         s.found_before = at;
         s.found_count = tie;
       }
       at += own;
-      tie += sums.ties[c];
+      tie += chunk_ties[c];
     }
     __syncthreads();
     const unsigned long long base = s.found_before;

@@ -165,6 +165,19 @@ struct Batch {
 // registers to hold them.
 constexpr uint32_t kStepBytes = 64 * kRowThreads;
 
+// A unit that is not wholly the row's, element by element (u = ~0: nothing of it is). Out of line: few units need it.
+template <class T>
+__device__ __noinline__ void fill_edge(const RowWalk<T> walk, uint32_t u, uint32_t at) {
+  float f[kUnit<T>];
+#pragma unroll
+  for (uint32_t i = 0; i < kUnit<T>; ++i) {
+    const uint32_t p = u * kUnit<T> + i;
+    f[i] = u != ~0u && p >= walk.head && p < walk.end ? walk.at(p) : -INFINITY;
+  }
+  const uint4 r = pack<T>(f);
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
+}
+
 template <class T, uint32_t kDepth>
 class Ring {
  public:
@@ -174,7 +187,7 @@ class Ring {
   __device__ __forceinline__ Ring(void* memory, const RowWalk<T>& walk, uint32_t first, uint32_t last)
       : walk_(walk), last_(last), ahead_(first), slot_(0) {
     mine_ = (uint32_t)__cvta_generic_to_shared(memory) + threadIdx.x * 16;
-#pragma unroll
+#pragma unroll 1
     for (uint32_t d = 0; d < kDepth; ++d) fill(d);
   }
   // Every copy has landed; the memory may be used for something else behind a barrier.
@@ -209,19 +222,11 @@ class Ring {
 #pragma unroll
       for (uint32_t j = 0; j < B::kUnits; ++j) {
         const uint32_t u = B::unit(u0, j);
-        if (inside || (u < last_ && walk_.whole(u))) {
+        if (inside || (u < last_ && walk_.whole(u)))
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(slot, j)), "l"(reinterpret_cast<const uint4*>(walk_.aligned) + u)
                        : "memory");
-        } else {
-          float f[kUnit<T>];
-#pragma unroll
-          for (uint32_t i = 0; i < kUnit<T>; ++i) {
-            const uint32_t p = u * kUnit<T> + i;
-            f[i] = u < last_ && p >= walk_.head && p < walk_.end ? walk_.at(p) : -INFINITY;
-          }
-          const uint4 r = pack<T>(f);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at(slot, j)), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
-        }
+        else
+          fill_edge<T>(walk_, u < last_ ? u : ~0u, at(slot, j));
       }
     }
     ahead_ = u0 + B::kSpan;
@@ -300,11 +305,6 @@ struct Soft {
       m = top;
     }
     s += step_sum(b, m, c);
-  }
-  __device__ __forceinline__ void merge(float m2, float s2, float c) {
-    const float top = fmaxf(m, m2);
-    s = s * (m == top ? 1.f : ex2((m - top) * c)) + s2 * (m2 == top ? 1.f : ex2((m2 - top) * c));
-    m = top;
   }
 };
 
@@ -418,9 +418,14 @@ __device__ __forceinline__ void tell_soft(const RowCluster& cluster, const Soft&
 }
 __device__ __forceinline__ Soft told_soft(const RowCluster& cluster, float c, const float2* slots) {
   Soft r;
-  r.m = slots[0].x;
-  r.s = slots[0].y;
-  for (uint32_t b = 1; b < cluster.blocks; ++b) r.merge(slots[b].x, slots[b].y, c);
+  float2 v[RowCluster::kMost];
+#pragma unroll
+  for (uint32_t b = 0; b < RowCluster::kMost; ++b) {
+    v[b] = b < cluster.blocks ? slots[b] : make_float2(-INFINITY, 0.f);
+    r.m = fmaxf(r.m, v[b].x);
+  }
+#pragma unroll
+  for (uint32_t b = 0; b < RowCluster::kMost; ++b) r.s += v[b].y * (v[b].x == r.m ? 1.f : ex2((v[b].x - r.m) * c));
   return r;
 }
 
