@@ -178,33 +178,31 @@ __device__ __noinline__ void sort_largest(TopShared& s, uint64_t* list, uint32_t
   const uint32_t t = threadIdx.x, places = n <= kSorted / 2 ? kSorted / 2 : kSorted;
   __syncthreads();
   uint64_t a = 2 * t < n ? list[2 * t] : 0, b = 2 * t + 1 < n ? list[2 * t + 1] : 0;
+#pragma unroll 1
   for (uint32_t size = 2; size <= places; size *= 2) {
     const bool down = (2 * t & size) == 0;
-    for (uint32_t far = size / 2; far; far /= 2) {
-      uint64_t oa, ob;
-      if (far == 1) {
-        if ((a < b) == down) {
-          const uint64_t c = a;
-          a = b;
-          b = c;
-        }
-        continue;
-      }
-      if (far <= 32) {
-        oa = __shfl_xor_sync(0xFFFFFFFFu, a, far / 2);
-        ob = __shfl_xor_sync(0xFFFFFFFFu, b, far / 2);
-      } else {
-        __syncthreads();
-        list[t] = a;
-        list[kRowThreads + t] = b;
-        __syncthreads();
-        oa = list[t ^ (far / 2)];
-        ob = list[kRowThreads + (t ^ (far / 2))];
-      }
+#pragma unroll 1
+    for (uint32_t far = size / 2; far > 32; far /= 2) {
+      __syncthreads();
+      list[t] = a;
+      list[kRowThreads + t] = b;
+      __syncthreads();
+      const uint64_t oa = list[t ^ (far / 2)], ob = list[kRowThreads + (t ^ (far / 2))];
       const bool larger = ((2 * t & far) == 0) == down;
       a = (a > oa) == larger ? a : oa;
       b = (b > ob) == larger ? b : ob;
     }
+#pragma unroll
+    for (uint32_t far = 32; far > 1; far /= 2) {
+      if (far >= size) continue;
+      const uint64_t oa = __shfl_xor_sync(0xFFFFFFFFu, a, far / 2), ob = __shfl_xor_sync(0xFFFFFFFFu, b, far / 2);
+      const bool larger = ((2 * t & far) == 0) == down;
+      a = (a > oa) == larger ? a : oa;
+      b = (b > ob) == larger ? b : ob;
+    }
+    const uint64_t high = a > b ? a : b, low = a > b ? b : a;
+    a = down ? high : low;
+    b = down ? low : high;
   }
   if (2 * t < k) s.sorted[2 * t] = a;
   if (2 * t + 1 < k) s.sorted[2 * t + 1] = b;
@@ -509,6 +507,12 @@ struct SampleSettings {
   }
 };
 
+// The tokens that may still be kept, if they are in `list`; all of the block's part otherwise.
+struct Few {
+  const uint64_t* list = nullptr;
+  uint32_t n = 0;
+};
+
 // A row under its temperature; one block's part of it, in units [first, last).
 template <class T>
 struct SampleRow {
@@ -521,13 +525,14 @@ struct SampleRow {
   // log2 of a token's weight.
   __device__ __forceinline__ double log_weight(float v) const { return v == m ? 0.0 : ((double)v - (double)m) * log2_t; }
   // 2^(y + 42) rounded to an integer, y <= 0. With n / 16 next to y, 2^y = 2^(n / 16) 2^f with |f| <= 1/32, and 2^f
-  // is e^(f ln 2) by its series up to the 6th power, off by 5e-16. Adding 2^10 leaves the multiple of 2^-42 in the sum's lower bits.
+  // is e^(f ln 2) by its series up to the 6th power, off by 5e-16. Adding 2^10 leaves the multiple of 2^-42 in the sum's
+  // lower bits. No branch, so that several go on at once: it is 13 operations in 64 bits, one behind the other.
   __device__ __forceinline__ unsigned long long fixed(double y) const {
-    if (!(y > -44.0)) return 0;
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: behind it a sum has no fraction
-    const double k = fma(y, 16.0, kRound);
+    const double z = fmax(y, -44.0);
+    const double k = fma(z, 16.0, kRound);
     const int n = __double2loint(k);
-    const double g = fma(k - kRound, -1.0 / 16, y) * 0.693147180559945309417;
+    const double g = fma(k - kRound, -1.0 / 16, z) * 0.693147180559945309417;
     double p = 1.0 / 720;
     p = fma(p, g, 1.0 / 120);
     p = fma(p, g, 1.0 / 24);
@@ -536,40 +541,43 @@ struct SampleRow {
     p = fma(p, g, 1.0);
     p = fma(p, g, 1.0) * roots[n & 15];
     p = __hiloint2double(__double2hiint(p) + (n >> 4) * (1 << 20), __double2loint(p)) + 1024.0;
-    return (unsigned long long)(__double_as_longlong(p) - __double_as_longlong(1024.0));
+    const unsigned long long w = (unsigned long long)(__double_as_longlong(p) - __double_as_longlong(1024.0));
+    return y > -44.0 ? w : 0;  // 2^-44 rounds to 0
   }
+  __device__ __forceinline__ unsigned long long fixed_of(float v) const { return fixed(log_weight(v)); }
   // As it counts when the token is drawn.
   __device__ __forceinline__ unsigned long long kept(float v, const SampleSettings& p) const {
     const double y = log_weight(v);
-    if (!(y >= p.log_min_p)) return 0;
-    const unsigned long long w = fixed(y);
-    return p.first() && w == 0 && y > -1075.0 ? 1 : w;
+    unsigned long long w = fixed(y);
+    if (p.first() && w == 0 && y > -1075.0) w = 1;
+    return y >= p.log_min_p ? w : 0;
   }
-  // visit(logit, id) for every logit of the block's part above -inf, or for those in `list`, where there is one. Four units a thread are
-  // on their way at once.
+  // visit(logits, id) for the units of the block's part, or for the candidates in `few`, where there are some: an array of logits,
+  // those that are not there as -inf, and a function from its index to a token's id. Four units a thread are on their way at once.
   template <class F>
-  __device__ __forceinline__ void each(const uint64_t* list, uint32_t n, F&& visit) const {
-    if (list) {
-      for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) visit(candidate_value(list[i]), 0xFFFFFFFFu - (uint32_t)list[i]);
+  __device__ __forceinline__ void each(const Few& few, F&& visit) const {
+    if (few.list) {
+      for (uint32_t i = threadIdx.x; i < few.n; i += kRowThreads) {
+        const float f[1] = {candidate_value(few.list[i])};
+        visit(f, [&](uint32_t) { return 0xFFFFFFFFu - (uint32_t)few.list[i]; });
+      }
       return;
     }
     for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
-      float f[Batch<T>::kUnits][kUnit<T>];
+      uint4 raw[Batch<T>::kUnits];
+      const bool inside = u0 * kUnit<T> >= walk.head && u0 + Batch<T>::kSpan <= last && (u0 + Batch<T>::kSpan) * kUnit<T> <= walk.end;
 #pragma unroll
       for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
         const uint32_t u = Batch<T>::unit(u0, j);
-        if (u < last) {
-          walk.load(u, f[j]);
-        } else {
-#pragma unroll
-          for (uint32_t i = 0; i < kUnit<T>; ++i) f[j][i] = -INFINITY;
-        }
+        raw[j] = inside ? __ldg(reinterpret_cast<const uint4*>(walk.aligned) + u) : load_edge(walk, u < last ? u : ~0u);
       }
 #pragma unroll
-      for (uint32_t j = 0; j < Batch<T>::kUnits; ++j)
-#pragma unroll
-        for (uint32_t i = 0; i < kUnit<T>; ++i)
-          if (f[j][i] > -INFINITY) visit(f[j][i], Batch<T>::unit(u0, j) * kUnit<T> + i - walk.head);
+      for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+        float f[kUnit<T>];
+        unpack<T>(raw[j], f);
+        const uint32_t id = Batch<T>::unit(u0, j) * kUnit<T> - walk.head;
+        visit(f, [&](uint32_t i) { return id + i; });
+      }
     }
   }
 };
@@ -613,29 +621,13 @@ __device__ __forceinline__ void find_in_chunk(SampleShared& s, const SampleRow<T
   }
 }
 
-// Sum over the cluster; every thread of it gets it.
-__device__ __forceinline__ unsigned long long cluster_sum(unsigned long long v, SampleShared& s) {
-  cg::cluster_group cluster = cg::this_cluster();
-  v = block_sum(v, s.scan);
-  if (threadIdx.x == 0) s.mine.mass = v;
-  cluster.sync();
-  unsigned long long t = 0;
-  for (uint32_t b = 0; b < cluster.num_blocks(); ++b) t += cluster.map_shared_rank(&s, b)->mine.mass;
-  cluster.sync();
-  return t;
-}
-
-// The tokens that may still be kept, if they are in `list`; all of the block's part otherwise.
-struct Few {
-  const uint64_t* list = nullptr;
-  uint32_t n = 0;
-};
-
 // One counting pass: digit(logit) in [0, kBins) for those that take part, or -1; in every bin how many they are and, where
-// `weigh`, their weight. Finds the lowest digit at which the running total (of counts, or of weights where
-// `weigh`) reaches `target`: s.found_*. The last bin, which may take most of a row, is counted in registers.
-template <class T, class D>
-__device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, const Few& few, bool weigh, unsigned long long target, D&& digit) {
+// `weigh`, their weight. Finds the lowest digit at which the running total (of counts, or of weights where `weigh`) reaches
+// target(total of all): s.found_*. A target of 0 asks for none. Returns the total. The last bin, which may take most of a row, is
+// counted in registers.
+template <class T, class D, class G>
+__device__ __forceinline__ unsigned long long find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, const Few& few, bool weigh,
+                                                       G&& target, D&& digit) {
   cg::cluster_group cluster = cg::this_cluster();
   for (uint32_t i = threadIdx.x; i < kBins; i += kRowThreads) {
     bins.count[i] = 0;
@@ -644,17 +636,28 @@ __device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, c
   __syncthreads();
   uint32_t tail_count = 0;
   unsigned long long tail_mass = 0;
-  row.each(few.list, few.n, [&](float v, uint32_t) {
-    const int d = digit(v);
-    if (d < 0) return;
-    const unsigned long long w = weigh ? row.fixed(row.log_weight(v)) : 0;
-    if (d == (int)kBins - 1) {
-      ++tail_count;
-      tail_mass += w;
-    } else {
-      atomicAdd(&bins.count[d], 1u);
-      if (w) atomicAdd(&bins.mass[d], w);
+  row.each(few, [&](const auto& f, auto) {
+    constexpr uint32_t n = sizeof(f) / sizeof(float);
+    int d[n];
+#pragma unroll
+    for (uint32_t i = 0; i < n; ++i) {
+      d[i] = digit(f[i]);
+      tail_count += d[i] == (int)kBins - 1;
     }
+    if (weigh) {
+      unsigned long long w[n];
+#pragma unroll
+      for (uint32_t i = 0; i < n; ++i) {
+        w[i] = row.fixed_of(f[i]);
+        tail_mass += d[i] == (int)kBins - 1 ? w[i] : 0;
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < n; ++i)
+        if ((uint32_t)d[i] < kBins - 1 && w[i]) atomicAdd(&bins.mass[d[i]], w[i]);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < n; ++i)
+      if ((uint32_t)d[i] < kBins - 1) atomicAdd(&bins.count[d[i]], 1u);
   });
   tail_count = (uint32_t)block_sum((unsigned long long)tail_count, s.scan);
   tail_mass = block_sum(tail_mass, s.scan);
@@ -679,10 +682,11 @@ __device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, c
     sum += weigh ? mass[j] : count[j];
   }
   unsigned long long before = block_scan(sum, s.scan, &all);
+  const unsigned long long goal = target(all);
 #pragma unroll
   for (uint32_t j = 0; j < kMine; ++j) {
     const unsigned long long in = weigh ? mass[j] : count[j];
-    if (before < target && before + in >= target) {
+    if (before < goal && before + in >= goal) {
       s.found_bin = threadIdx.x * kMine + j;
       s.found_before = before;
       s.found_count = count[j];
@@ -690,42 +694,57 @@ __device__ void find_bin(SampleShared& s, Bins& bins, const SampleRow<T>& row, c
     before += in;
   }
   cluster.sync();  // found_* is there, and no block reads these bins any more
+  return all;
 }
 
-// The logit at which the total over the row in descending order reaches `target` (1 <= target <= the
-// total), among logits above `floor`, and how many of the tokens with this very logit it takes.
-template <class T>
-__device__ Kept find_edge(SampleShared& s, ExactShared& m, const SampleRow<T>& row, Few& few, bool weigh, unsigned long long target, float floor) {
+// The logit at which the total over the row in descending order reaches `target`, among logits above `floor`, and how many of the tokens
+// with this very logit it takes. target(total of all above the floor) is at most that total; where it is 0, there is no edge to find and
+// `kept` stays.
+template <class T, class G>
+__device__ __forceinline__ void find_edge(SampleShared& s, ExactShared& m, const SampleRow<T>& row, Few& few, bool weigh, float floor,
+                                          Kept& kept, G&& target) {
   cg::cluster_group cluster = cg::this_cluster();
-  Bins& bins = m.bins;
   // First by distance from the maximum, 1/64 of a temperature a bin and one for all that is 16 below.
   const float scale = fminf((float)(64.0 * row.inv_t), 3e38f);
   auto coarse = [&](float v) { return v == row.m ? 0 : (int)fminf((row.m - v) * scale, (float)(kBins - 1)); };
-  find_bin(s, bins, row, few, weigh, target, [&](float v) { return v > floor ? coarse(v) : -1; });
+  unsigned long long goal = 0;
+  find_bin(s, m.bins, row, few, weigh, [&](unsigned long long all) { return goal = target(all); }, [&](float v) { return v > floor ? coarse(v) : -1; });
+  if (goal == 0) return;  // the same for the whole cluster
   const int bin = (int)s.found_bin;
-  target -= s.found_before;
+  goal -= s.found_before;
   uint32_t at = s.found_count;
   // Nothing below this bin is kept: if what is above is few in this block, the passes to come need not go over the row.
+  // The edge lies above the floor, so that tokens at the floor itself are not kept. The list has the counts of up to kBins chunks beside it.
   if (!few.list) {
     if (threadIdx.x == 0) s.top.count = 0;
     __syncthreads();
-    row.each(nullptr, 0, [&](float v, uint32_t id) {
-      if (v > floor && coarse(v) <= bin) {
-        const uint32_t i = atomicAdd(&s.top.count, 1u);
-        if (i < kCandidates) m.list[i] = candidate(v, id);
+    row.each(few, [&](const auto& f, auto id) {
+      constexpr uint32_t n = sizeof(f) / sizeof(float);
+      uint32_t mask = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < n; ++i) mask |= (f[i] > floor && coarse(f[i]) <= bin ? 1u : 0u) << i;
+      if (!mask) return;
+      uint32_t i0 = atomicAdd(&s.top.count, (uint32_t)__popc(mask));
+#pragma unroll
+      for (uint32_t i = 0; i < n; ++i) {
+        if (mask >> i & 1u) {
+          if (i0 < kCandidates) m.list[i0] = candidate(f[i], id(i));
+          ++i0;
+        }
       }
     });
     __syncthreads();
-    // The edge lies above the floor, so that tokens at the floor itself are not kept. The list has the counts of up to kBins chunks beside it.
     if (s.top.count <= kCandidates && row.last - row.first <= kBins * kChunkUnits) few = Few{m.list, s.top.count};
   }
   // Then by the order keys of the bin's logits, from the first bit in which they differ.
   uint32_t lo = 0xFFFFFFFFu, hi = 0;
-  row.each(few.list, few.n, [&](float v, uint32_t) {
-    if (v > floor && coarse(v) == bin) {
-      const uint32_t k = order_key(v);
-      lo = min(lo, k);
-      hi = max(hi, k);
+  row.each(few, [&](const auto& f, auto) {
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(f) / sizeof(float); ++i) {
+      const bool in = f[i] > floor && coarse(f[i]) == bin;
+      const uint32_t k = order_key(f[i]);
+      lo = min(lo, in ? k : 0xFFFFFFFFu);
+      hi = max(hi, in ? k : 0u);
     }
   });
   lo = __reduce_min_sync(0xFFFFFFFFu, lo);
@@ -749,27 +768,25 @@ __device__ Kept find_edge(SampleShared& s, ExactShared& m, const SampleRow<T>& r
   cluster.sync();
   int left = lo == hi ? 0 : 32 - __clz(lo ^ hi);  // low bits still open
   uint32_t prefix = left == 32 ? 0 : hi >> left;  // those above
+#pragma unroll 1
   while (left > 0) {
     const int step = min(left, 8);
     const int shift = left - step;
     // The largest digit first: digits are counted from the top.
-    find_bin(s, bins, row, few, weigh, target, [&](float v) {
-      if (!(v > floor) || coarse(v) != bin) return -1;
+    find_bin(s, m.bins, row, few, weigh, [&](unsigned long long) { return goal; }, [&](float v) {
       const uint32_t k = order_key(v);
-      if (left < 32 && (k >> left) != prefix) return -1;
-      return (int)((1u << step) - 1u - ((k >> shift) & ((1u << step) - 1u)));
+      const bool in = v > floor && coarse(v) == bin && (left == 32 || (k >> left) == prefix);
+      return in ? (int)((1u << step) - 1u - ((k >> shift) & ((1u << step) - 1u))) : -1;
     });
-    target -= s.found_before;
+    goal -= s.found_before;
     at = s.found_count;
     prefix = (left == 32 ? 0u : prefix << step) | ((1u << step) - 1u - s.found_bin);
     left = shift;
     __syncthreads();  // found_* is read
   }
-  Kept kept;
   kept.edge = key_value(prefix);
-  const unsigned long long one = row.fixed(row.log_weight(kept.edge));
-  kept.ties = weigh ? (uint32_t)min((unsigned long long)at, (target + one - 1) / max(one, 1ull)) : (uint32_t)target;
-  return kept;
+  const unsigned long long one = row.fixed_of(kept.edge);
+  kept.ties = weigh ? (uint32_t)min((unsigned long long)at, (goal + one - 1) / max(one, 1ull)) : (uint32_t)goal;
 }
 
 // The row's token from integer weights of all its tokens, by the whole cluster: into s.token of the block that holds it.
@@ -784,22 +801,22 @@ __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const Sa
     kept.edge = row.m;
     kept.ties = 1;
   } else if (p.top_k > 1 && p.top_k < (int64_t)vocab) {
-    unsigned long long there = 0;
-    row.each(nullptr, 0, [&](float, uint32_t) { ++there; });
-    if (cluster_sum(there, s) > (unsigned long long)p.top_k) kept = find_edge(s, m, row, few, false, (unsigned long long)p.top_k, -INFINITY);
+    const unsigned long long most = (unsigned long long)p.top_k;
+    find_edge(s, m, row, few, false, -INFINITY, kept, [&](unsigned long long all) { return all > most ? most : 0; });
   }
   if (p.top_p < 1.f && p.top_k != 1) {
-    unsigned long long above = 0;
-    row.each(few.list, few.n, [&](float v, uint32_t) { above += v > kept.edge ? row.fixed(row.log_weight(v)) : 0; });
-    above = cluster_sum(above, s);
-    const unsigned long long one = kept.edge > -INFINITY ? row.fixed(row.log_weight(kept.edge)) : 0;
-    const unsigned long long total = above + one * kept.ties;
-    unsigned long long target = (unsigned long long)ceil((double)p.top_p * (double)total);
-    target = min(max(target, 1ull), total);
-    if (target > above)
-      kept.ties = min(kept.ties, (uint32_t)((target - above + one - 1) / max(one, 1ull)));
-    else
-      kept = find_edge(s, m, row, few, true, target, kept.edge);
+    const float floor = kept.edge;
+    const unsigned long long one = floor > -INFINITY ? row.fixed_of(floor) : 0;
+    uint32_t ties = kept.ties;
+    find_edge(s, m, row, few, true, floor, kept, [&](unsigned long long above) {
+      const unsigned long long total = above + one * ties;
+      unsigned long long goal = (unsigned long long)ceil((double)p.top_p * (double)total);
+      goal = min(max(goal, 1ull), total);
+      if (goal <= above) return goal;
+      ties = min(ties, (uint32_t)((goal - above + one - 1) / max(one, 1ull)));  // it ends among those at the floor
+      return 0ull;
+    });
+    if (kept.edge == floor) kept.ties = ties;
   }
 
   // Weights of the tokens kept, in id order: by chunks, then within the chunk that holds the token.
@@ -820,8 +837,9 @@ __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const Sa
       chunk_ties[c] = 0;
     }
     __syncthreads();
-    row.each(few.list, few.n, [&](float v, uint32_t id) {
-      const uint32_t c = (id + row.walk.head) / kChunk<T> - chunk0;
+    for (uint32_t i = threadIdx.x; i < few.n; i += kRowThreads) {
+      const float v = candidate_value(few.list[i]);
+      const uint32_t c = (0xFFFFFFFFu - (uint32_t)few.list[i] + row.walk.head) / kChunk<T> - chunk0;
       if (v > kept.edge) {
         const unsigned long long w = row.kept(v, p);
         atomicAdd(&chunk_mass[c], w);
@@ -830,28 +848,28 @@ __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const Sa
         atomicAdd(&chunk_ties[c], 1u);
         ++tied;
       }
-    });
+    }
   } else {
     for (uint32_t ch = chunk0 + warp; ch < chunk1; ch += kRowWarps) {
       unsigned long long w = 0;
       uint32_t e = 0;
-      float f[Batch<T>::kUnits][kUnit<T>];
+      uint4 raw[Batch<T>::kUnits];
+      const uint32_t u0 = ch * kChunkUnits;
+      const bool inside = u0 * kUnit<T> >= row.walk.head && u0 + kChunkUnits <= row.last && (u0 + kChunkUnits) * kUnit<T> <= row.walk.end;
 #pragma unroll
       for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
-        const uint32_t u = ch * kChunkUnits + j * 32 + lane;
-        if (u < row.last) {
-          row.walk.load(u, f[j]);
-        } else {
-#pragma unroll
-          for (uint32_t i = 0; i < kUnit<T>; ++i) f[j][i] = -INFINITY;
-        }
+        const uint32_t u = u0 + j * 32 + lane;
+        raw[j] = inside ? __ldg(reinterpret_cast<const uint4*>(row.walk.aligned) + u) : load_edge(row.walk, u < row.last ? u : ~0u);
       }
 #pragma unroll
       for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+        float f[kUnit<T>];
+        unpack<T>(raw[j], f);
 #pragma unroll
         for (uint32_t i = 0; i < kUnit<T>; ++i) {
-          if (f[j][i] > kept.edge) w += row.kept(f[j][i], p);
-          e += edged && f[j][i] == kept.edge;
+          const unsigned long long one_w = row.kept(f[i], p);
+          w += f[i] > kept.edge ? one_w : 0;
+          e += edged && f[i] == kept.edge;
         }
       }
 #pragma unroll

@@ -165,17 +165,17 @@ struct Batch {
 // registers to hold them.
 constexpr uint32_t kStepBytes = 64 * kRowThreads;
 
-// A unit that is not wholly the row's, element by element (u = ~0: nothing of it is). Out of line: few units need it.
+// A unit that may not be wholly the row's, element by element where it is not (u = ~0: nothing of it is). Out of line: few units need it.
 template <class T>
-__device__ __noinline__ void fill_edge(const RowWalk<T> walk, uint32_t u, uint32_t at) {
+__device__ __noinline__ uint4 load_edge(const RowWalk<T> walk, uint32_t u) {
   float f[kUnit<T>];
+  if (u == ~0u) {
 #pragma unroll
-  for (uint32_t i = 0; i < kUnit<T>; ++i) {
-    const uint32_t p = u * kUnit<T> + i;
-    f[i] = u != ~0u && p >= walk.head && p < walk.end ? walk.at(p) : -INFINITY;
+    for (uint32_t i = 0; i < kUnit<T>; ++i) f[i] = -INFINITY;
+  } else {
+    walk.load(u, f);
   }
-  const uint4 r = pack<T>(f);
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
+  return pack<T>(f);
 }
 
 template <class T, uint32_t kDepth>
@@ -222,11 +222,13 @@ class Ring {
 #pragma unroll
       for (uint32_t j = 0; j < B::kUnits; ++j) {
         const uint32_t u = B::unit(u0, j);
-        if (inside || (u < last_ && walk_.whole(u)))
+        if (inside || (u < last_ && walk_.whole(u))) {
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(slot, j)), "l"(reinterpret_cast<const uint4*>(walk_.aligned) + u)
                        : "memory");
-        else
-          fill_edge<T>(walk_, u < last_ ? u : ~0u, at(slot, j));
+        } else {
+          const uint4 r = load_edge(walk_, u < last_ ? u : ~0u);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at(slot, j)), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
+        }
       }
     }
     ahead_ = u0 + B::kSpan;
