@@ -30,6 +30,7 @@ constexpr uint32_t kFewMaxima = 64;
 constexpr uint32_t kCandidates = WS_TOP_MAX_K + kRowThreads * 8;
 constexpr uint32_t kCounted = 128;  // candidates that are put in order by counting
 constexpr uint32_t kSorted = 512;   // and by sorting
+constexpr uint32_t kMostCollected = 1200;  // of 4096 maxima in a row of 16 groups: 1420 logits reach the bound; of 2048: 1810
 
 struct TopShared {
   uint64_t sorted[WS_TOP_MAX_K];  // the block's k largest in order
@@ -236,14 +237,19 @@ struct TopCollector {
       if (--left == 0) close();
     }
   }
-  // Behind the last step: s.sorted_count (at most k) candidates in s.sorted, in order; visible behind the next barrier. `list`:
-  // room for kCandidates that the ring has left.
-  __device__ __forceinline__ void finish(uint64_t* list, const RowWalk<T>& walk, uint32_t first, uint32_t last) {
+  // Behind the last step: the k largest, and some others that come close, in `list`, room for kCandidates that the ring has left; s.count of
+  // them (more than kCandidates: not all were written down). k up to kMostCollected.
+  __device__ __forceinline__ float collect(uint64_t* list, const RowWalk<T>& walk, uint32_t first, uint32_t last) {
     if (left != each) close();
     if (threadIdx.x == 0) s.count = s.queued = 0;
     uint16_t* queue = reinterpret_cast<uint16_t*>(list + kCandidates);
     float bound;
-    if (k > kFewMaxima) {
+    if (k > WS_TOP_MAX_K) {
+      float every[kGroups];
+#pragma unroll
+      for (uint32_t g = 0; g < kGroups; ++g) every[g] = g < group ? fmaxf(key_value((uint32_t)s.maxima[g][threadIdx.x] << 16), -INFINITY) : -INFINITY;
+      bound = kth_of_maxima(s, every, k);
+    } else if (k > kFewMaxima) {
       bound = kth_of_maxima(s, most, k);
     } else {
       const float one[1] = {fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))};
@@ -268,6 +274,11 @@ struct TopCollector {
       }
     }
     __syncthreads();
+    return bound;
+  }
+  // s.sorted_count (at most k <= WS_TOP_MAX_K) candidates in s.sorted, in order; visible behind the next barrier.
+  __device__ __forceinline__ void finish(uint64_t* list, const RowWalk<T>& walk, uint32_t first, uint32_t last) {
+    const float bound = collect(list, walk, first, last);
     if (s.count > kCandidates) top_by_units<T>(s, list, walk, first, last, k, bound);
     if (s.count > kSorted) keep_largest(s, list, s.count, k);  // k <= WS_TOP_MAX_K <= kSorted remain
     const uint32_t n = s.count;
@@ -357,7 +368,7 @@ __device__ __forceinline__ void tell_top(const RowCluster& cluster, const TopSha
 }
 
 template <class T>
-__global__ void __launch_bounds__(kRowThreads, 3)
+__global__ void __launch_bounds__(kRowThreads, 4)
     top_kernel(RowSet x, uint32_t k, float c, float inv_t, int64_t* __restrict__ ids, float* __restrict__ logprobs) {
   // The ring, and behind it, where the row has several blocks, what they tell each other.
   extern __shared__ __align__(16) uint8_t memory[];
@@ -790,12 +801,11 @@ __device__ __forceinline__ void find_edge(SampleShared& s, ExactShared& m, const
 }
 
 // The row's token from integer weights of all its tokens, by the whole cluster: into s.token of the block that holds it.
-// `memory`: what the ring left, for the counts.
+// `memory`: what the ring left, for the counts. `few`: the block's part of the first top-k, if they are known.
 template <class T>
-__device__ __noinline__ void exact_token(SampleShared& s, void* memory, const SampleRow<T>& row, const SampleSettings& p, uint32_t vocab) {
+__device__ __noinline__ void exact_token(SampleShared& s, void* memory, const SampleRow<T>& row, const SampleSettings& p, Few few, uint32_t vocab) {
   cg::cluster_group cluster = cg::this_cluster();
   ExactShared& m = *reinterpret_cast<ExactShared*>(memory);
-  Few few;
   Kept kept;
   if (p.top_k == 1) {
     kept.edge = row.m;
@@ -990,7 +1000,7 @@ __device__ __forceinline__ bool token_of_largest(SampleShared& s, const SampleRo
 }
 
 template <class T>
-__global__ void __launch_bounds__(kRowThreads, 2)
+__global__ void __launch_bounds__(kRowThreads, 3)
     sample_kernel(RowSet x, const float* __restrict__ uniform, ws_sampling sampling, int64_t* __restrict__ tokens,
                   float* __restrict__ logprobs) {
   // The ring (then what exact_token counts), (m, s) of the row's chunks, and, where the row has several blocks, what they tell each other.
@@ -1012,7 +1022,11 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   TopTold* told = reinterpret_cast<TopTold*>(soft + ((chunks + 1) & ~1u));
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const bool dropping = (p.top_k >= 1 && p.top_k < (int64_t)x.vocab) || p.top_p < 1.f || p.min_p > 0.f;
-  const uint32_t k = p.top_k >= 1 && p.top_k <= WS_TOP_MAX_K ? (uint32_t)p.top_k : WS_TOP_MAX_K;
+  // The largest logits, in order: as many as top-k asks for, or WS_TOP_MAX_K. A larger top-k is left to exact_token, which up to
+  // kMostCollected gets a list.
+  const bool many = p.top_k > WS_TOP_MAX_K && p.top_k <= kMostCollected && p.top_k < (int64_t)x.vocab;
+  const uint32_t k = p.top_k >= 1 && p.top_k <= kMostCollected ? (uint32_t)p.top_k : WS_TOP_MAX_K;
+  Few few;
 
   Ring<T, kTopDepth> ring(memory, walk, row.first, row.last);
   TopCollector<T> top(s.top, k, row.first, row.last);
@@ -1036,10 +1050,18 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     if (dropping) top.add(most, all);
     ring.advance();
   }
-  if (dropping) top.finish(reinterpret_cast<uint64_t*>(memory), walk, row.first, row.last);
+  if (many) {
+    uint64_t* candidates = reinterpret_cast<ExactShared*>(memory)->list;
+    top.collect(candidates, walk, row.first, row.last);
+    // The list has the counts of up to kBins chunks beside it.
+    if (s.top.count <= kCandidates && row.last - row.first <= kBins * kChunkUnits) few = Few{candidates, s.top.count};
+  } else if (dropping) {
+    top.finish(reinterpret_cast<uint64_t*>(memory), walk, row.first, row.last);
+  }
   __syncthreads();
   const uint64_t* list = s.top.sorted;
-  uint32_t n = dropping ? s.top.sorted_count : 0;
+  const bool sorted = dropping && !many;
+  uint32_t n = sorted ? s.top.sorted_count : 0;
   if (cluster.blocks > 1) {
     cluster.ready();
     for (uint32_t b = 0; b < cluster.blocks; ++b) {
@@ -1047,9 +1069,9 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       float2* to = cluster.of(soft, b);
       for (uint32_t i = chunk0 + threadIdx.x; i < chunk1; i += kRowThreads) to[i] = soft[i];
     }
-    if (dropping) tell_top(cluster, s.top, told);
+    if (sorted) tell_top(cluster, s.top, told);
     cluster.told();
-    if (dropping) {
+    if (sorted) {
       const uint32_t own = n;
       n = 0;
       for (uint32_t b = 0; b < cluster.blocks; ++b) n += told->counts[b];
@@ -1095,9 +1117,9 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     if (threadIdx.x == 0) s.token = ((uint64_t)(0xFFFFFFFFu - (uint32_t)list[0]) << 32) | (list[0] >> 32);
     decided = true;
   } else if (isfinite(total) && c < 1e30f) {
-    if (dropping) {
+    if (sorted) {
       decided = token_of_largest(s, row, p, list, n, all_there, x.vocab, total);
-    } else if (!p.first()) {
+    } else if (!dropping && !p.first()) {
       const double target = p.u * total;
       if (threadIdx.x == 0) s.chunk = chunks;
       __syncthreads();
@@ -1126,7 +1148,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   const bool here = decided;
   if (!decided) {
     __syncthreads();
-    exact_token(s, memory, row, p, x.vocab);
+    exact_token(s, memory, row, p, few, x.vocab);
   } else {
     __syncthreads();
   }
