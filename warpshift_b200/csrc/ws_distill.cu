@@ -61,20 +61,23 @@ struct Record {
 constexpr uint32_t kDepth = 3;      // steps in flight of the kernels that read a row once
 constexpr uint32_t kStepDepth = 4;  // of the one that reads it twice: a block's share up to 64 KiB stays
 
-// Entry `threadIdx.x` of a row's record and the logit of its token; a token id of -1 has no mass.
+// Entry `threadIdx.x` of a row's record and the logit of its token; a token id of -1 has no mass. Loaded in two parts, the second of
+// which needs the first, so that a kernel can read its row in between.
 struct Entry {
   int id = -1;
   float lp = -INFINITY, x = 0.f;
+  int64_t raw = -1;
 
-  template <class T>
-  __device__ __forceinline__ void load(const Record& r, uint32_t row, const T* logits, uint32_t vocab) {
+  __device__ __forceinline__ void load(const Record& r, uint32_t row) {
     if (threadIdx.x >= r.k) return;
     const size_t at = (size_t)row * r.k + threadIdx.x;
-    const int64_t raw = r.ids32 ? ((const int32_t*)r.ids)[at] : ((const int64_t*)r.ids)[at];
-    const float l = r.logprobs[at];
-    if (raw >= 0 && raw < (int64_t)vocab && l > -INFINITY) {
+    raw = r.ids32 ? ((const int32_t*)r.ids)[at] : ((const int64_t*)r.ids)[at];
+    lp = r.logprobs[at];
+  }
+  template <class T>
+  __device__ __forceinline__ void look_up(const T* logits, uint32_t vocab) {
+    if (raw >= 0 && raw < (int64_t)vocab && lp > -INFINITY) {
       id = (int)raw;
-      lp = l;
       x = to_float(logits[raw]);
     }
   }
@@ -234,25 +237,28 @@ __global__ void __launch_bounds__(kRowThreads, 4)
   __shared__ float2 soft_scratch[kRowWarps], soft_slots[RowCluster::kMost];
   __shared__ RecordSums part[kRowWarps];
   const RowCluster cluster;
+  cluster.started();
   const uint32_t row = cluster.row();
   const float w = r.weights ? r.weights[row] : 1.f;
+  Entry e;
+  if (cluster.rank == 0) e.load(r, row);
   float2* out = reinterpret_cast<float2*>(stats) + row;
-  if (w == 0.f) {  // the same for the whole cluster
+  const T* src = row_ptr<T>(x, row);
+  const RowWalk<T> walk(src, x.vocab);
+  uint32_t first, last;
+  split_units(walk.units, cluster.rank, cluster.blocks, first, last);
+  Ring<T, kDepth> ring(ring_memory, walk, first, last);  // on its way before the weight is there
+  if (w == 0.f) {                                        // the same for the whole cluster
+    ring.drain();
+    cluster.ready();
     if (cluster.rank == 0 && threadIdx.x == 0) {
       loss[row] = 0.f;
       *out = make_float2(0.f, 0.f);
     }
     return;
   }
-  cluster.started();
-  const T* src = row_ptr<T>(x, row);
-  const RowWalk<T> walk(src, x.vocab);
-  uint32_t first, last;
-  split_units(walk.units, cluster.rank, cluster.blocks, first, last);
-  Ring<T, kDepth> ring(ring_memory, walk, first, last);
-  if (cluster.rank == 0) {  // while the first copies are on their way
-    Entry e;
-    e.load(r, row, src, x.vocab);
+  if (cluster.rank == 0) {
+    e.look_up(src, x.vocab);
     sum_record(r, e, part);
   }
   Soft soft = row_soft(ring, first, last, r.c, soft_scratch);
@@ -281,20 +287,23 @@ __global__ void __launch_bounds__(kRowThreads, 4)
   const float w = r.weights ? r.weights[row] : 1.f;
   const float2 st = reinterpret_cast<const float2*>(stats)[row];
   const uint32_t o = row / x.inner, in = row - o * x.inner;
-  const float g = grad_loss[(int64_t)o * grad_outer + (int64_t)in * grad_inner] * w * r.inv_t;
+  const float out_g = grad_loss[(int64_t)o * grad_outer + (int64_t)in * grad_inner];
+  Entry e;
+  e.load(r, row);
   const T* src = row_ptr<T>(x, row);
   const RowWalk<T> walk(src, x.vocab);
   uint32_t first, last;
   split_units(walk.units, cluster.rank, cluster.blocks, first, last);
   T* out = row_ptr<T>(dx, row) - walk.head;  // by aligned position
   const bool wide = ((uintptr_t)out & 15u) == 0;
+  Ring<T, kDepth> ring(ring_memory, walk, first, last);  // on its way before the factors are there
+  const float g = out_g * w * r.inv_t;
   if (w == 0.f || g == 0.f || st.y == 0.f) {
+    ring.drain();
     write_zeros(walk, out, wide, first, last);
     return;
   }
-  Ring<T, kDepth> ring(ring_memory, walk, first, last);
-  Entry e;
-  e.load(r, row, src, x.vocab);
+  e.look_up(src, x.vocab);
   if (r.renormalize) sum_record(r, e, part);
   const float a = g * st.y;
   for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
@@ -323,23 +332,26 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   __shared__ GradShared s;
   __shared__ RowGrad shared_grad;
   const RowCluster cluster;
+  cluster.started();
   const uint32_t row = cluster.row();
   const float w = r.weights ? r.weights[row] : 1.f;
+  Entry e;
+  e.load(r, row);
   const T* src = row_ptr<T>(x, row);
   const RowWalk<T> walk(src, x.vocab);
   uint32_t first, last;
   split_units(walk.units, cluster.rank, cluster.blocks, first, last);
   T* out = row_ptr<T>(dx, row) - walk.head;
   const bool wide = ((uintptr_t)out & 15u) == 0;
-  if (w == 0.f) {  // the same for the whole cluster
+  Ring<T, kStepDepth> ring(ring_memory, walk, first, last);  // on its way before the weight is there
+  if (w == 0.f) {                                            // the same for the whole cluster
+    ring.drain();
+    cluster.ready();
     if (cluster.rank == 0 && threadIdx.x == 0) loss[row] = 0.f;
     write_zeros(walk, out, wide, first, last);
     return;
   }
-  cluster.started();
-  Ring<T, kStepDepth> ring(ring_memory, walk, first, last);
-  Entry e;
-  e.load(r, row, src, x.vocab);
+  e.look_up(src, x.vocab);
   sum_record(r, e, part);
   Soft soft = row_soft(ring, first, last, r.c, soft_scratch);
   if (cluster.blocks > 1) {

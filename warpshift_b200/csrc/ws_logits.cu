@@ -224,13 +224,14 @@ struct TopCollector {
 #pragma unroll
     for (uint32_t j = 0; j < B::kUnits; ++j) most[j] = -INFINITY;
   }
-  // The next step, by the largest of the thread's logits in each unit and in all of them.
-  __device__ __forceinline__ void add(const float (&top)[B::kUnits], float all) {
+  // The next step; all: the largest of the thread's logits in it.
+  __device__ __forceinline__ void add(const B& b, float all) {
     if (each == 0) {
 #pragma unroll
       for (uint32_t j = 0; j < B::kUnits; ++j) {
-        most[j] = fmaxf(most[j], top[j]);
-        put(top[j]);
+        const float top = word_top<T>(unit_word<T>(b.raw[j]));
+        most[j] = fmaxf(most[j], top);
+        put(top);
       }
     } else {
       here = fmaxf(here, all);
@@ -385,14 +386,9 @@ __global__ void __launch_bounds__(kRowThreads, 4)
   for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
     Batch<T> b;
     ring.read(b);
-    float most[Batch<T>::kUnits], all = -INFINITY;
-#pragma unroll
-    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
-      most[j] = unit_max<T>(b.raw[j]);
-      all = fmaxf(all, most[j]);
-    }
+    const float all = step_max(b);
     soft.add(b, all, c);
-    top.add(most, all);
+    top.add(b, all);
     ring.advance();
   }
   top.finish(reinterpret_cast<uint64_t*>(memory), walk, first, last);
@@ -1035,19 +1031,14 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   for (uint32_t u0 = row.first; u0 < row.last; u0 += Batch<T>::kSpan) {
     Batch<T> b;
     ring.read(b);
-    float most[Batch<T>::kUnits], all = -INFINITY;
-#pragma unroll
-    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
-      most[j] = unit_max<T>(b.raw[j]);
-      all = fmaxf(all, most[j]);
-    }
+    const float all = step_max(b);
     const float m = key_value(__reduce_max_sync(0xFFFFFFFFu, order_key(all)));
     float sum = step_sum(b, m, c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     const uint32_t ch = u0 / kChunkUnits + warp;
     if (lane == 0 && ch < chunk1) soft[ch] = make_float2(m, sum);
-    if (dropping) top.add(most, all);
+    if (dropping) top.add(b, all);
     ring.advance();
   }
   if (many) {

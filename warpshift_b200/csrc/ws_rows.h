@@ -187,6 +187,12 @@ class Ring {
   __device__ __forceinline__ Ring(void* memory, const RowWalk<T>& walk, uint32_t first, uint32_t last)
       : walk_(walk), last_(last), ahead_(first), slot_(0) {
     mine_ = (uint32_t)__cvta_generic_to_shared(memory) + threadIdx.x * 16;
+    source_ = reinterpret_cast<const uint4*>(walk.aligned) + B::unit(first, 0);
+    // Steps that begin from inside_from_ to inside_to_ are wholly the row's and the range's.
+    inside_from_ = walk.head ? 1 : 0;
+    const uint32_t whole = min(last, walk.end / kUnit<T>);
+    inside_to_ = whole >= B::kSpan ? whole - B::kSpan : 0;
+    if (whole < B::kSpan) inside_from_ = ~0u;
 #pragma unroll 1
     for (uint32_t d = 0; d < kDepth; ++d) fill(d);
   }
@@ -216,27 +222,32 @@ class Ring {
     }
   }
   __device__ __forceinline__ void fill(uint32_t slot) {
-    const uint32_t u0 = ahead_;
-    if (u0 < last_) {
-      const bool inside = u0 * kUnit<T> >= walk_.head && u0 + B::kSpan <= last_ && (u0 + B::kSpan) * kUnit<T> <= walk_.end;
+    if (ahead_ < last_) {
+      if (ahead_ >= inside_from_ && ahead_ <= inside_to_) {
 #pragma unroll
-      for (uint32_t j = 0; j < B::kUnits; ++j) {
-        const uint32_t u = B::unit(u0, j);
-        if (inside || (u < last_ && walk_.whole(u))) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(slot, j)), "l"(reinterpret_cast<const uint4*>(walk_.aligned) + u)
-                       : "memory");
-        } else {
+        for (uint32_t j = 0; j < B::kUnits; ++j)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(slot, j)), "l"(source_ + j * 32) : "memory");
+      } else {
+#pragma unroll 1
+        for (uint32_t j = 0; j < B::kUnits; ++j) {
+          const uint32_t u = B::unit(ahead_, j);
+          if (u < last_ && walk_.whole(u)) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(slot, j)), "l"(source_ + j * 32) : "memory");
+            continue;
+          }
           const uint4 r = load_edge(walk_, u < last_ ? u : ~0u);
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at(slot, j)), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
         }
       }
     }
-    ahead_ = u0 + B::kSpan;
+    ahead_ += B::kSpan;
+    source_ += B::kSpan;
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
   const RowWalk<T>& walk_;
-  uint32_t last_, ahead_, slot_, mine_;
+  const uint4* source_;
+  uint32_t last_, ahead_, slot_, mine_, inside_from_, inside_to_;
 };
 
 // Pairs of fp32 in one instruction.
@@ -431,14 +442,42 @@ __device__ __forceinline__ Soft told_soft(const RowCluster& cluster, float c, co
   return r;
 }
 
+// The larger of two words' elements, a NaN giving way to a number: two elements in one instruction where they have 16 bits.
 template <class T>
-__device__ __forceinline__ float unit_max(const uint4& r) {
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t word_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <>
+__device__ __forceinline__ uint32_t word_max<__half>(uint32_t a, uint32_t b) {
+  const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <>
+__device__ __forceinline__ uint32_t word_max<float>(uint32_t a, uint32_t b) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+template <class T>
+__device__ __forceinline__ uint32_t unit_word(const uint4& r) {
+  return word_max<T>(word_max<T>(r.x, r.y), word_max<T>(r.z, r.w));
+}
+// The largest element of a word; -inf if there is no number.
+template <class T>
+__device__ __forceinline__ float word_top(uint32_t w) {
+  if (sizeof(T) == 4) return fmaxf(__uint_as_float(w), -INFINITY);
   float f[kUnit<T>];
-  unpack<T>(r, f);
-  float top = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+  unpack<T>(make_uint4(w, w, w, w), f);
+  return fmaxf(fmaxf(f[0], f[1]), -INFINITY);
+}
+// The largest of a thread's logits in a step.
+template <class T>
+__device__ __forceinline__ float step_max(const Batch<T>& b) {
+  uint32_t w = unit_word<T>(b.raw[0]);
 #pragma unroll
-  for (uint32_t i = 4; i < kUnit<T>; i += 2) top = fmaxf(top, fmaxf(f[i], f[i + 1]));
-  return top;
+  for (uint32_t j = 1; j < Batch<T>::kUnits; ++j) w = word_max<T>(w, unit_word<T>(b.raw[j]));
+  return word_top<T>(w);
 }
 
 // Statistics of the units that `ring` reads, for the whole block.
@@ -448,10 +487,7 @@ __device__ __forceinline__ Soft row_soft(Ring<T, kDepth>& ring, uint32_t first, 
   for (uint32_t u = first; u < last; u += Batch<T>::kSpan) {
     Batch<T> b;
     ring.read(b);
-    float top = unit_max<T>(b.raw[0]);
-#pragma unroll
-    for (uint32_t j = 1; j < Batch<T>::kUnits; ++j) top = fmaxf(top, unit_max<T>(b.raw[j]));
-    soft.add(b, top, c);
+    soft.add(b, step_max(b), c);
     ring.advance();
   }
   return block_soft(soft, c, scratch);
