@@ -88,8 +88,8 @@ struct Entry {
 // the teacher's tail neither underflows nor overflows, and logits relative to the largest one of the record, so that
 // nothing is lost where logits are huge (a mask of the type's lowest value).
 struct RecordSums {
-  double q = 0.0, q_lp = 0.0, q_x = 0.0;  // sums of q, q lp and q (x - at), q = exp(lp - shift)
-  float shift = 0.f, at = 0.f;
+  double q, q_lp, q_x;  // sums of q, q lp and q (x - at), q = exp(lp - shift)
+  float shift, at;
 
   __device__ __forceinline__ void merge(const RecordSums& o) {
     if (o.q == 0.0) return;
@@ -107,10 +107,20 @@ struct RecordSums {
   }
 };
 
-// The warp's part of the record into `part` (one slot for each warp).
-__device__ __forceinline__ void sum_record(const Record& r, const Entry& e, RecordSums* part) {
+// A row's record as the block's threads share it.
+struct RecordShared {
+  RecordSums part[kRowWarps];
+  int ids[WS_TOP_MAX_K];
+  float lps[WS_TOP_MAX_K];
+};
+
+// The thread's entry and, where asked for, the warp's part of the sums into `s`; a barrier has to follow.
+__device__ __forceinline__ void put_record(const Record& r, const Entry& e, RecordShared& s, bool sums = true) {
   const uint32_t warp = threadIdx.x >> 5;
-  RecordSums t;
+  s.ids[threadIdx.x] = e.id;
+  s.lps[threadIdx.x] = e.lp;
+  if (!sums) return;
+  RecordSums t{0.0, 0.0, 0.0, 0.f, 0.f};
   if (warp * 32 < r.k) {
     const uint32_t none = order_key(-INFINITY);
     if (r.renormalize) {
@@ -131,67 +141,130 @@ __device__ __forceinline__ void sum_record(const Record& r, const Entry& e, Reco
       t.q_x += __shfl_xor_sync(0xFFFFFFFFu, t.q_x, o);
     }
   }
-  if ((threadIdx.x & 31u) == 0) part[warp] = t;
+  if ((threadIdx.x & 31u) == 0) s.part[warp] = t;
 }
 
-// What the gradient of a row needs: (mass / S) exp((x_i - m) / t) for the dense part, scale exp(lp - shift) for
-// the record's. Both 0: the row has no gradient, and its logits are not read for it.
+__device__ __forceinline__ RecordSums record_sums(const Record& r, const RecordShared& s) {
+  RecordSums t = s.part[0];
+  for (uint32_t w = 1; w * 32 < r.k; ++w) t.merge(s.part[w]);
+  return t;
+}
+
+// The first entry that names a token writes its gradient: for that thread, the sum of exp(lp - its own lp) over all entries that name it;
+// 0 for the others and for tokens outside units [first, last).
+template <class T>
+__device__ __forceinline__ float record_share(const Record& r, const Entry& e, const RecordShared& s, const RowWalk<T>& walk, uint32_t first,
+                                              uint32_t last) {
+  const uint32_t p = (uint32_t)e.id + walk.head;
+  if (e.id < 0 || p < first * kUnit<T> || p >= last * kUnit<T>) return 0.f;
+  float share = 0.f;
+  bool owner = true;
+#pragma unroll 4
+  for (uint32_t j = 0; j < r.k; ++j) {
+    if (s.ids[j] == e.id) {
+      owner = owner && j >= threadIdx.x;
+      share += j == threadIdx.x ? 1.f : expf(s.lps[j] - e.lp);
+    }
+  }
+  return owner ? share : 0.f;
+}
+
+// What the gradient of a row needs: dense * 2^((x_i - m) c) for every token, and record * exp(lp - shift) less for those on record. dense = 0: the
+// row has no gradient, and its logits are not read for it.
 struct RowGrad {
-  float m = 0.f, mass_over_s = 0.f, scale = 0.f, shift = 0.f;
+  float m = 0.f, dense = 0.f, record = 0.f, shift = 0.f;
 };
 
-// The row's loss before its weight, and the gradient's factors. One thread's work.
-__device__ __forceinline__ float finish_loss(const Record& r, const RecordSums* part, const Soft& soft, RowGrad& g) {
-  RecordSums t = part[0];
-  for (uint32_t w = 1; w * 32 < r.k; ++w) t.merge(part[w]);
-  g = RowGrad{};
-  if (t.q == 0.0) return 0.f;                // no mass on record
-  if (soft.m == -INFINITY) return INFINITY;  // no finite logit
+__device__ __forceinline__ RowGrad row_grad(const Record& r, const RecordSums& t, const Soft& soft, float factor) {
+  RowGrad g;
+  if (t.q == 0.0 || soft.m == -INFINITY) return g;
   g.m = soft.m;
   g.shift = t.shift;
-  const double scale = r.renormalize ? 1.0 / t.q : 1.0;
-  g.scale = (float)scale;
-  g.mass_over_s = (float)(t.q * scale / (double)soft.s);
+  g.dense = factor * (r.renormalize ? 1.f / soft.s : (float)(t.q / (double)soft.s));
+  g.record = r.renormalize ? (float)((double)factor / t.q) : factor;
+  return g;
+}
+
+// The row's loss before its weight.
+__device__ __forceinline__ float row_loss(const Record& r, const RecordSums& t, const Soft& soft) {
+  if (t.q == 0.0) return 0.f;                // no mass on record
+  if (soft.m == -INFINITY) return INFINITY;  // no finite logit
   const double log_s = log((double)soft.s);
   const double q_d = (t.q_x + t.q * ((double)t.at - (double)soft.m)) * (double)r.inv_t;
-  if (r.renormalize) return (float)((t.q_lp - q_d) * scale - (log(t.q) + (double)t.shift) + log_s);
+  if (r.renormalize) return (float)((t.q_lp - q_d) / t.q - (log(t.q) + (double)t.shift) + log_s);
   return (float)(t.q_lp - q_d + t.q * log_s);
 }
 
-struct GradShared {
-  int ids[WS_TOP_MAX_K];
-  float qs[WS_TOP_MAX_K];
-};
-
-// One step's units of a gradient row: a 2^((x - m) c), or zeros.
+// A unit of a gradient row element by element, what lies outside the row left alone.
 template <class T>
-__device__ __forceinline__ void write_step(const RowWalk<T>& walk, T* out, bool wide, uint32_t u0, uint32_t last, const Batch<T>& b,
-                                           float m, float c, float a) {
-  const uint64_t nm = pair(-m, -m), cc = pair(c, c), aa = pair(a, a);
+__device__ __noinline__ void write_edge(const RowWalk<T> walk, T* out, uint32_t u, uint4 v) {
+  float f[kUnit<T>];
+  unpack<T>(v, f);
 #pragma unroll
-  for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
-    const uint32_t u = Batch<T>::unit(u0, j);
-    if (u >= last) continue;
-    float f[kUnit<T>];
-    unpack<T>(b.raw[j], f);
-#pragma unroll
-    for (uint32_t i = 0; i < kUnit<T>; i += 2) {
-      const float2 e = unpair(mul2(add2(pair(f[i], f[i + 1]), nm), cc));
-      const float2 g = unpair(mul2(aa, pair(ex2(e.x), ex2(e.y))));
-      f[i] = g.x;
-      f[i + 1] = g.y;
-    }
-    if (wide && walk.whole(u)) {
-      reinterpret_cast<uint4*>(out)[u] = pack<T>(f);
-    } else {
-#pragma unroll
-      for (uint32_t i = 0; i < kUnit<T>; ++i) {
-        const uint32_t p = u * kUnit<T> + i;
-        if (p >= walk.head && p < walk.end) out[p] = from_float<T>(f[i]);
-      }
-    }
+  for (uint32_t i = 0; i < kUnit<T>; ++i) {
+    const uint32_t p = u * kUnit<T> + i;
+    if (p >= walk.head && p < walk.end) out[p] = from_float<T>(f[i]);
   }
 }
+
+// The dense part of a gradient row, a 2^((x - m) c).
+template <class T>
+class DenseGrad {
+ public:
+  __device__ __forceinline__ DenseGrad(const RowWalk<T>& walk, T* out, uint32_t last, const RowGrad& g, float c)
+      : walk_(walk), out_(out), last_(last), m_(g.m), c_(c), a_(g.dense) {
+    wide_ = ((uintptr_t)out & 15u) == 0;
+    r_ = m_ * c;
+    scale_ = a_ * one_step_rest(m_, c, r_);
+    one_step_ = one_step(m_, c);
+    // For 16-bit gradients the factor goes into the exponent, which is off by 2^-24 of 200 at most then, 8e-6 of the value: far below
+    // their own rounding.
+    folded_ = sizeof(T) == 2 && a_ > 1e-30f && a_ < 1e30f && fabsf(r_) < 100.f;
+    if (folded_) r_ -= log2f(scale_);
+  }
+  // One step's units, which begin at unit u0; inside: they are wholly the row's.
+  __device__ __forceinline__ void write(const Batch<T>& b, uint32_t u0, bool inside) const {
+    uint4* out = reinterpret_cast<uint4*>(out_) + Batch<T>::unit(u0, 0);
+    const uint64_t cc = pair(c_, c_), nr = pair(-r_, -r_), aa = pair(scale_, scale_);
+#pragma unroll
+    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+      float f[kUnit<T>];
+      unpack<T>(b.raw[j], f);
+      if (one_step_) {
+#pragma unroll
+        for (uint32_t i = 0; i < kUnit<T>; i += 2) {
+          const float2 e = unpair(fma2(pair(f[i], f[i + 1]), cc, nr));
+          f[i] = ex2(e.x);
+          f[i + 1] = ex2(e.y);
+        }
+        if (!folded_) {
+#pragma unroll
+          for (uint32_t i = 0; i < kUnit<T>; i += 2) {
+            const float2 e = unpair(mul2(pair(f[i], f[i + 1]), aa));
+            f[i] = e.x;
+            f[i + 1] = e.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kUnit<T>; ++i) f[i] = a_ * ex2((f[i] - m_) * c_);
+      }
+      const uint4 v = pack<T>(f);
+      const uint32_t u = Batch<T>::unit(u0, j);
+      if (wide_ && (inside || (u < last_ && walk_.whole(u))))
+        out[j * 32] = v;
+      else if (u < last_)
+        write_edge(walk_, out_, u, v);
+    }
+  }
+
+ private:
+  const RowWalk<T>& walk_;
+  T* out_;
+  uint32_t last_;
+  float m_, c_, a_, r_, scale_;
+  bool wide_, one_step_, folded_;
+};
 
 template <class T>
 __device__ __forceinline__ void write_zeros(const RowWalk<T>& walk, T* out, bool wide, uint32_t first, uint32_t last) {
@@ -208,26 +281,12 @@ __device__ __forceinline__ void write_zeros(const RowWalk<T>& walk, T* out, bool
   }
 }
 
-// The elements of units [first, last) that the record names, behind the dense part: each once, by the first entry that names it.
+// The element that the thread's entry names, if it is its to write; behind the dense part.
 template <class T>
-__device__ __forceinline__ void write_record(const Record& r, const Entry& e, const RowWalk<T>& walk, T* out, uint32_t first,
-                                             uint32_t last, const RowGrad& g, float a, float b, GradShared& s) {
-  s.ids[threadIdx.x] = e.id;
-  s.qs[threadIdx.x] = e.id >= 0 ? expf(e.lp - g.shift) : 0.f;
-  __syncthreads();  // the block's dense part is written, too
-  const uint32_t p = (uint32_t)e.id + walk.head;
-  if (e.id >= 0 && p >= first * kUnit<T> && p < last * kUnit<T>) {
-    float q = 0.f;
-    bool owner = true;
-#pragma unroll 4
-    for (uint32_t j = 0; j < r.k; ++j) {
-      if (s.ids[j] == e.id) {
-        owner = owner && j >= threadIdx.x;
-        q += s.qs[j];
-      }
-    }
-    if (owner) out[p] = from_float<T>(a * ex2((e.x - g.m) * r.c) - b * q);
-  }
+__device__ __forceinline__ void write_record(const Record& r, const Entry& e, float share, const RowWalk<T>& walk, T* out, const RowGrad& g) {
+  __syncthreads();  // the block's dense part is written
+  if (share != 0.f)
+    out[(uint32_t)e.id + walk.head] = from_float<T>(g.dense * ex2((e.x - g.m) * r.c) - g.record * (share * expf(e.lp - g.shift)));
 }
 
 template <class T>
@@ -235,7 +294,7 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     distill_forward_kernel(RowSet x, Record r, float* __restrict__ loss, float* __restrict__ stats) {
   extern __shared__ __align__(16) uint8_t ring_memory[];
   __shared__ float2 soft_scratch[kRowWarps], soft_slots[RowCluster::kMost];
-  __shared__ RecordSums part[kRowWarps];
+  __shared__ RecordShared record;
   const RowCluster cluster;
   cluster.started();
   const uint32_t row = cluster.row();
@@ -257,11 +316,9 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     }
     return;
   }
-  if (cluster.rank == 0) {
-    e.look_up(src, x.vocab);
-    sum_record(r, e, part);
-  }
-  Soft soft = row_soft(ring, first, last, r.c, soft_scratch);
+  Soft soft = read_soft(ring, first, last, r.c, [&] { e.look_up(src, x.vocab); });
+  if (cluster.rank == 0) put_record(r, e, record);
+  soft = block_soft(soft, r.c, soft_scratch);
   if (cluster.blocks > 1) {
     cluster.ready();
     tell_soft(cluster, soft, soft_slots);
@@ -269,9 +326,10 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     soft = told_soft(cluster, r.c, soft_slots);
   }
   if (cluster.rank == 0 && threadIdx.x == 0) {
-    RowGrad g;
-    loss[row] = w * finish_loss(r, part, soft, g);
-    *out = make_float2(g.m, g.mass_over_s);
+    const RecordSums t = record_sums(r, record);
+    loss[row] = w * row_loss(r, t, soft);
+    const RowGrad g = row_grad(r, t, soft, 1.f);
+    *out = make_float2(g.m, g.dense);
   }
 }
 
@@ -280,8 +338,7 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     distill_backward_kernel(RowSet x, Record r, const float* __restrict__ stats, const float* __restrict__ grad_loss,
                             int64_t grad_outer, int64_t grad_inner, RowSet dx) {
   extern __shared__ __align__(16) uint8_t ring_memory[];
-  __shared__ GradShared s;
-  __shared__ RecordSums part[kRowWarps];
+  __shared__ RecordShared record;
   const RowCluster cluster;  // its blocks have nothing to tell each other here
   const uint32_t row = cluster.row();
   const float w = r.weights ? r.weights[row] : 1.f;
@@ -295,32 +352,32 @@ __global__ void __launch_bounds__(kRowThreads, 4)
   uint32_t first, last;
   split_units(walk.units, cluster.rank, cluster.blocks, first, last);
   T* out = row_ptr<T>(dx, row) - walk.head;  // by aligned position
-  const bool wide = ((uintptr_t)out & 15u) == 0;
+  const bool wide = ((uintptr_t)out & 15u) == 0;  // for rows without a gradient
   Ring<T, kDepth> ring(ring_memory, walk, first, last);  // on its way before the factors are there
-  const float g = out_g * w * r.inv_t;
-  if (w == 0.f || g == 0.f || st.y == 0.f) {
+  const float factor = out_g * w * r.inv_t;
+  if (w == 0.f || factor == 0.f || st.y == 0.f) {
     ring.drain();
     write_zeros(walk, out, wide, first, last);
     return;
   }
-  e.look_up(src, x.vocab);
-  if (r.renormalize) sum_record(r, e, part);
-  const float a = g * st.y;
+  RowGrad g{st.x, factor * st.y, factor, 0.f};
+  const DenseGrad<T> dense(walk, out, last, g, r.c);
   for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
     Batch<T> b;
     ring.read(b);
-    write_step(walk, out, wide, u0, last, b, st.x, r.c, a);
+    dense.write(b, u0, ring.inside(u0));
     ring.advance();
+    if (u0 == first) e.look_up(src, x.vocab);
   }
-  RowGrad f{st.x, st.y, 1.f, 0.f};
+  put_record(r, e, record, r.renormalize);
+  __syncthreads();
+  const float share = record_share(r, e, record, walk, first, last);
   if (r.renormalize) {
-    __syncthreads();
-    RecordSums t = part[0];
-    for (uint32_t i = 1; i * 32 < r.k; ++i) t.merge(part[i]);
-    f.scale = (float)(1.0 / t.q);
-    f.shift = t.shift;
+    const RecordSums t = record_sums(r, record);
+    g.record = (float)((double)factor / t.q);
+    g.shift = t.shift;
   }
-  write_record(r, e, walk, out, first, last, f, a, g * f.scale, s);
+  write_record(r, e, share, walk, out, g);
 }
 
 template <class T>
@@ -328,9 +385,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
     distill_step_kernel(RowSet x, Record r, float* __restrict__ loss, RowSet dx) {
   extern __shared__ __align__(16) uint8_t ring_memory[];
   __shared__ float2 soft_scratch[kRowWarps], soft_slots[RowCluster::kMost];
-  __shared__ RecordSums part[kRowWarps];
-  __shared__ GradShared s;
-  __shared__ RowGrad shared_grad;
+  __shared__ RecordShared record;
   const RowCluster cluster;
   cluster.started();
   const uint32_t row = cluster.row();
@@ -342,7 +397,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   uint32_t first, last;
   split_units(walk.units, cluster.rank, cluster.blocks, first, last);
   T* out = row_ptr<T>(dx, row) - walk.head;
-  const bool wide = ((uintptr_t)out & 15u) == 0;
+  const bool wide = ((uintptr_t)out & 15u) == 0;  // for rows without a gradient
   Ring<T, kStepDepth> ring(ring_memory, walk, first, last);  // on its way before the weight is there
   if (w == 0.f) {                                            // the same for the whole cluster
     ring.drain();
@@ -351,46 +406,41 @@ __global__ void __launch_bounds__(kRowThreads, 3)
     write_zeros(walk, out, wide, first, last);
     return;
   }
-  e.look_up(src, x.vocab);
-  sum_record(r, e, part);
-  Soft soft = row_soft(ring, first, last, r.c, soft_scratch);
+  Soft soft = read_soft(ring, first, last, r.c, [&] { e.look_up(src, x.vocab); });
+  put_record(r, e, record);
+  soft = block_soft(soft, r.c, soft_scratch);
   if (cluster.blocks > 1) {
     cluster.ready();
     tell_soft(cluster, soft, soft_slots);
-    cluster.told();
-    soft = told_soft(cluster, r.c, soft_slots);
   }
-  if (threadIdx.x == 0) {
-    RowGrad g;
-    const float l = w * finish_loss(r, part, soft, g);
-    if (cluster.rank == 0) loss[row] = l;
-    shared_grad = g;
-  }
-  __syncthreads();
-  const RowGrad g = shared_grad;
-  const float a = w * r.inv_t * g.mass_over_s, b = w * r.inv_t * g.scale;
-  if (g.mass_over_s == 0.f) {
+  cluster.telling();
+  const float share = record_share(r, e, record, walk, first, last);
+  const RecordSums t = record_sums(r, record);
+  cluster.heard();
+  if (cluster.blocks > 1) soft = told_soft(cluster, r.c, soft_slots);
+  const RowGrad g = row_grad(r, t, soft, w * r.inv_t);
+  const DenseGrad<T> dense(walk, out, last, g, r.c);
+  if (g.dense == 0.f) {
     write_zeros(walk, out, wide, first, last);
-    return;
-  }
-  // The second pass, from shared memory where the block's share is still there.
-  if (last - first <= kStepDepth * Batch<T>::kSpan) {
+  } else if (last - first <= kStepDepth * Batch<T>::kSpan) {
+    // The second pass from shared memory, where the block's share still is.
     uint32_t slot = 0;
     for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan, ++slot) {
-      Batch<T> t;
-      ring.again(slot, t);
-      write_step(walk, out, wide, u0, last, t, g.m, r.c, a);
+      Batch<T> b;
+      ring.again(slot, b);
+      dense.write(b, u0, ring.inside(u0));
     }
   } else {
     Ring<T, kStepDepth> second(ring_memory, walk, first, last);
     for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
-      Batch<T> t;
-      second.read(t);
-      write_step(walk, out, wide, u0, last, t, g.m, r.c, a);
+      Batch<T> b;
+      second.read(b);
+      dense.write(b, u0, ring.inside(u0));
       second.advance();
     }
   }
-  write_record(r, e, walk, out, first, last, g, a, b, s);
+  if (g.dense != 0.f) write_record(r, e, share, walk, out, g);
+  if (cluster.rank == 0 && threadIdx.x == 0) loss[row] = w * row_loss(r, t, soft);
 }
 
 int fail(int code, const std::string& msg) {
@@ -463,7 +513,7 @@ extern "C" int ws_distill_backward(const ws_rows* logits, const ws_teacher* teac
     if (x.rows == 0) return (int)WS_OK;
     if (!stats || !grad_loss) return fail(WS_ERR_INVALID, "null pointer");
     if ((uintptr_t)stats % 8) return fail(WS_ERR_INVALID, "stats must be 8-byte aligned");
-    const uint32_t pieces = blocks_a_row(x);
+    const uint32_t pieces = blocks_a_row(x, 56);
     DeviceGuard guard(device);
     cudaError_t e = guard.error();
     if (e == cudaSuccess)
@@ -492,7 +542,7 @@ extern "C" int ws_distill_step(const ws_rows* logits, const ws_teacher* teacher,
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows<distill_step_kernel<T>>(x.rows, blocks_a_row(x), kStepDepth * kStepBytes, device, stream, x.set, r, loss, dx.set);
+        return launch_rows<distill_step_kernel<T>>(x.rows, blocks_a_row(x, 96), kStepDepth * kStepBytes, device, stream, x.set, r, loss, dx.set);
       });
     return done(e, "distill step");
   });

@@ -206,6 +206,8 @@ class Ring {
   }
   // Step `slot` of the first kDepth, which stays where it is as long as no later step is copied over it.
   __device__ __forceinline__ void again(uint32_t slot, B& b) const { fetch(slot, b); }
+  // Whether all units of the block's step that begins at unit u0 are wholly the row's.
+  __device__ __forceinline__ bool inside(uint32_t u0) const { return u0 >= inside_from_ && u0 <= inside_to_; }
   // To the step after it; to be called when what read() gave has been used.
   __device__ __forceinline__ void advance() {
     fill(slot_);
@@ -223,7 +225,7 @@ class Ring {
   }
   __device__ __forceinline__ void fill(uint32_t slot) {
     if (ahead_ < last_) {
-      if (ahead_ >= inside_from_ && ahead_ <= inside_to_) {
+      if (inside(ahead_)) {
 #pragma unroll
         for (uint32_t j = 0; j < B::kUnits; ++j)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(slot, j)), "l"(source_ + j * 32) : "memory");
@@ -272,6 +274,12 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return v;
 }
 
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+
 // Floats as integers of the same order (-0 is taken as +0 first, so that equal
 // logits have equal keys).
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -282,24 +290,53 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+// 2^((x - m) c) takes one multiply-add before the exponential as 2^(x c - r), r = m c rounded, times 2^(r - m c), which is a constant near 1
+// that one more multiply-add gives exactly. x c - r is rounded once, so nothing is lost against (x - m) c; but r - m c has to be
+// small: with |m| c below kOneStep it is at most 64. Beyond (masks of the type's lowest value, temperatures next to 0) the difference
+// comes first.
+constexpr float kOneStep = 1e9f;
+__device__ __forceinline__ bool one_step(float m, float c) { return fabsf(m) * c < kOneStep; }
+__device__ __forceinline__ float one_step_rest(float m, float c, float r) { return ex2(-fmaf(m, c, -r)); }
+
 // Sum of 2^((x - m) c) over a thread's units of a step (m = -inf: all of them are -inf, and the sum is 0).
 template <class T>
 __device__ __forceinline__ float step_sum(const Batch<T>& b, float m, float c) {
   const float base = m == -INFINITY ? 0.f : m;
-  const uint64_t nb = pair(-base, -base), cc = pair(c, c);
+  const uint64_t cc = pair(c, c);
   uint64_t sum = 0;
+  float scale = 1.f;
+  if (one_step(base, c)) {
+    const float r = base * c;
+    const uint64_t nr = pair(-r, -r);
 #pragma unroll
-  for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
-    float f[kUnit<T>];
-    unpack<T>(b.raw[j], f);
+    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+      float f[kUnit<T>];
+      unpack<T>(b.raw[j], f);
 #pragma unroll
-    for (uint32_t i = 0; i < kUnit<T>; i += 2) {
-      const float2 e = unpair(mul2(add2(pair(f[i], f[i + 1]), nb), cc));
-      sum = add2(sum, pair(ex2(e.x), ex2(e.y)));
+      for (uint32_t i = 0; i < kUnit<T>; i += 2) {
+        const float2 e = unpair(fma2(pair(f[i], f[i + 1]), cc, nr));
+        sum = add2(sum, pair(ex2(e.x), ex2(e.y)));
+      }
+    }
+    scale = one_step_rest(base, c, r);
+  } else {
+    const uint64_t nb = pair(-base, -base);
+#pragma unroll 1
+    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+      uint4 raw = b.raw[0];
+#pragma unroll
+      for (uint32_t q = 1; q < Batch<T>::kUnits; ++q) raw = q == j ? b.raw[q] : raw;
+      float f[kUnit<T>];
+      unpack<T>(raw, f);
+#pragma unroll
+      for (uint32_t i = 0; i < kUnit<T>; i += 2) {
+        const float2 e = unpair(mul2(add2(pair(f[i], f[i + 1]), nb), cc));
+        sum = add2(sum, pair(ex2(e.x), ex2(e.y)));
+      }
     }
   }
   const float2 t = unpair(sum);
-  return t.x + t.y;
+  return (t.x + t.y) * scale;
 }
 
 // Running maximum m and sum s of 2^((x - m) c), c = log2(e) / temperature. The
@@ -408,12 +445,16 @@ class RowCluster {
     if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   __device__ __forceinline__ void told() const {
-    if (blocks > 1) {
-      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    } else {
-      __syncthreads();
-    }
+    telling();
+    heard();
+  }
+  // Its two halves, for work in between that touches none of what is told.
+  __device__ __forceinline__ void telling() const {
+    if (blocks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  }
+  __device__ __forceinline__ void heard() const {
+    if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();
   }
   // `p` of this block's shared memory, in block b's.
   template <class V>
@@ -480,17 +521,19 @@ __device__ __forceinline__ float step_max(const Batch<T>& b) {
   return word_top<T>(w);
 }
 
-// Statistics of the units that `ring` reads, for the whole block.
-template <class T, uint32_t kDepth>
-__device__ __forceinline__ Soft row_soft(Ring<T, kDepth>& ring, uint32_t first, uint32_t last, float c, float2* scratch) {
+// A thread's statistics of the units that `ring` reads. between(): called once, behind the first step, when what was loaded before the
+// ring has come in.
+template <class T, uint32_t kDepth, class F>
+__device__ __forceinline__ Soft read_soft(Ring<T, kDepth>& ring, uint32_t first, uint32_t last, float c, F&& between) {
   Soft soft;
   for (uint32_t u = first; u < last; u += Batch<T>::kSpan) {
     Batch<T> b;
     ring.read(b);
     soft.add(b, step_max(b), c);
     ring.advance();
+    if (u == first) between();
   }
-  return block_soft(soft, c, scratch);
+  return soft;
 }
 
 // Units of the row that block `rank` of `blocks` walks.
@@ -543,11 +586,14 @@ cudaError_t by_type(int dtype, F&& f) {
   }
 }
 
-// How many blocks (a cluster: 1, 2, 4 or 8) share each row.
-inline uint32_t blocks_a_row(const RowArgs& x) {
-  const uint32_t bytes = x.set.vocab * (x.dtype == WS_DTYPE_FP32 ? 4u : 2u);
+// How many blocks (a cluster: 1, 2, 4 or 8) share each row. Every block costs some microseconds beside its share of the row, so that
+// many rows go to one block each; kernels that write as much as they read gain from smaller shares, down to `share` KiB (0: one block).
+// Fewer rows than two blocks for each of 148 SMs are split until there are that many blocks, down to 16 KiB a block.
+inline uint32_t blocks_a_row(const RowArgs& x, uint32_t share = 0) {
+  const uint32_t kib = x.set.vocab / 1024 * (x.dtype == WS_DTYPE_FP32 ? 4u : 2u);
   uint32_t c = 1;
-  while (c < 8 && (uint64_t)x.rows * c * 2 <= 592 && bytes / c >= 8192) c *= 2;
+  while (c < 8 && share && kib >= 2 * c * share) c *= 2;
+  while (c < 8 && (uint64_t)x.rows * c * 2 <= 296 && kib >= 2 * c * 16) c *= 2;
   return c;
 }
 
