@@ -447,6 +447,7 @@ constexpr uint32_t kChunk = kChunkUnits * kUnit<T>;
 constexpr uint32_t kChunks = WS_MAX_VOCAB / kChunk<float> + 1;
 constexpr double kWeightOne = 4398046511104.0;  // 2^42
 constexpr double kSumError = 1.0 / 131072;
+constexpr double kNoWeight = -16.0 * 1075.0;  // 16 log2 of what 64 bits round to 0
 
 struct Bins {
   uint32_t count[kBins];
@@ -499,7 +500,7 @@ struct SampleSettings {
     min_p = fminf(p.min_p_each ? p.min_p_each[row] : p.min_p, 1.f);
     top_k = top_k_of(p, row);
     u = (double)uniform[row];
-    log_min_p = min_p > 0.f ? log2((double)min_p) : -INFINITY;
+    log_min_p = min_p > 0.f ? 16.0 * log2((double)min_p) : 0.0;
     if (!(t > 0.f)) {
       t = 1.f;
       top_k = 1;
@@ -526,38 +527,44 @@ struct SampleRow {
   RowWalk<T> walk;
   uint32_t first, last;
   float m;
-  double inv_t, log2_t;  // 1 and log2(e) over the temperature
+  double inv_t, log2_t, log2_m;  // 1 and 16 log2(e) over the temperature, and the latter times -m
   const double* roots;   // 2^(i / 16) for i from 0 to 15
 
-  // log2 of a token's weight.
-  __device__ __forceinline__ double log_weight(float v) const { return v == m ? 0.0 : ((double)v - (double)m) * log2_t; }
-  // 2^(y + 42) rounded to an integer, y <= 0. With n / 16 next to y, 2^y = 2^(n / 16) 2^f with |f| <= 1/32, and 2^f
-  // is e^(f ln 2) by its series up to the 6th power, off by 5e-16. Adding 2^10 leaves the multiple of 2^-42 in the sum's
-  // lower bits. No branch, so that several go on at once: it is 13 operations in 64 bits, one behind the other.
+  // 16 log2 of a token's weight. In 64 bits nothing is lost by taking the products before the difference: logits that are not equal differ by
+  // 2^-24 of their size, the products are off by 2^-53 of it.
+  __device__ __forceinline__ double log_weight(float v) const {
+    // v in 64 bits by its bits, which are quicker than a conversion; 0 and what lies next to it become 2^-127, infinities 2^128.
+    const uint32_t u = __float_as_uint(v);
+    const double x = __hiloint2double((int)((u & 0x80000000u) | ((u & 0x7FFFFFFFu) >> 3) + 0x38000000u), (int)(u << 29));
+    return v == m ? 0.0 : fma(x, log2_t, log2_m);
+  }
+  // 2^(y / 16 + 42) rounded to an integer, y <= 0. With n next to y, 2^(y / 16) = 2^(n / 16) 2^(f / 16) with |f| <= 1/2, and 2^(f / 16) is
+  // e^(f ln 2 / 16) by its series up to the 5th power, off by 2e-13, less than 2^-42. Adding 2^10 leaves the multiple of 2^-42 in the sum's
+  // lower bits. No branch, so that several go on at once: it is 12 operations in 64 bits, one behind the other.
   __device__ __forceinline__ unsigned long long fixed(double y) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: behind it a sum has no fraction
-    const double z = fmax(y, -44.0);
-    const double k = fma(z, 16.0, kRound);
+    constexpr double kStep = 0.693147180559945309417 / 16;
+    const double k = y + kRound;
     const int n = __double2loint(k);
-    const double g = fma(k - kRound, -1.0 / 16, z) * 0.693147180559945309417;
-    double p = 1.0 / 720;
-    p = fma(p, g, 1.0 / 120);
-    p = fma(p, g, 1.0 / 24);
-    p = fma(p, g, 1.0 / 6);
-    p = fma(p, g, 0.5);
-    p = fma(p, g, 1.0);
-    p = fma(p, g, 1.0) * roots[n & 15];
+    const double f = y - (k - kRound);
+    double p = kStep * kStep * kStep * kStep * kStep / 120;
+    p = fma(p, f, kStep * kStep * kStep * kStep / 24);
+    p = fma(p, f, kStep * kStep * kStep / 6);
+    p = fma(p, f, kStep * kStep / 2);
+    p = fma(p, f, kStep);
+    p = fma(p, f, 1.0) * roots[n & 15];
     p = __hiloint2double(__double2hiint(p) + (n >> 4) * (1 << 20), __double2loint(p)) + 1024.0;
     const unsigned long long w = (unsigned long long)(__double_as_longlong(p) - __double_as_longlong(1024.0));
-    return y > -44.0 ? w : 0;  // 2^-44 rounds to 0
+    return y > -704.0 ? w : 0;  // 2^-44 rounds to 0
   }
   __device__ __forceinline__ unsigned long long fixed_of(float v) const { return fixed(log_weight(v)); }
   // As it counts when the token is drawn.
   __device__ __forceinline__ unsigned long long kept(float v, const SampleSettings& p) const {
     const double y = log_weight(v);
     unsigned long long w = fixed(y);
-    if (p.first() && w == 0 && y > -1075.0) w = 1;
-    return y >= p.log_min_p ? w : 0;
+    if (p.first() && w == 0 && y > kNoWeight) w = 1;
+    if (p.min_p > 0.f && !(y >= p.log_min_p)) w = 0;
+    return w;
   }
   // visit(logits, id) for the units of the block's part, or for the candidates in `few`, where there are some: an array of logits,
   // those that are not there as -inf, and a function from its index to a token's id. Four units a thread are on their way at once.
@@ -720,16 +727,18 @@ __device__ __forceinline__ void find_edge(SampleShared& s, ExactShared& m, const
   const int bin = (int)s.found_bin;
   goal -= s.found_before;
   uint32_t at = s.found_count;
-  // Nothing below this bin is kept: if what is above is few in this block, the passes to come need not go over the row.
-  // The edge lies above the floor, so that tokens at the floor itself are not kept. The list has the counts of up to kBins chunks beside it.
-  if (!few.list) {
+  // Nothing below this bin is kept: if what is above is few in this block, the passes to come need not go over the row; if only the bin's own
+  // tokens are, those of this function need not. The edge lies above the floor, so that tokens at the floor itself are not kept. The list has
+  // the counts of up to kBins chunks beside it.
+  Few in_bin = few;
+  for (int only = 0; only < 2 && !in_bin.list; ++only) {
     if (threadIdx.x == 0) s.top.count = 0;
     __syncthreads();
     row.each(few, [&](const auto& f, auto id) {
       constexpr uint32_t n = sizeof(f) / sizeof(float);
       uint32_t mask = 0;
 #pragma unroll
-      for (uint32_t i = 0; i < n; ++i) mask |= (f[i] > floor && coarse(f[i]) <= bin ? 1u : 0u) << i;
+      for (uint32_t i = 0; i < n; ++i) mask |= (f[i] > floor && (only ? coarse(f[i]) == bin : coarse(f[i]) <= bin) ? 1u : 0u) << i;
       if (!mask) return;
       uint32_t i0 = atomicAdd(&s.top.count, (uint32_t)__popc(mask));
 #pragma unroll
@@ -741,11 +750,13 @@ __device__ __forceinline__ void find_edge(SampleShared& s, ExactShared& m, const
       }
     });
     __syncthreads();
-    if (s.top.count <= kCandidates && row.last - row.first <= kBins * kChunkUnits) few = Few{m.list, s.top.count};
+    if (s.top.count <= kCandidates) in_bin = Few{m.list, s.top.count};
+    if (in_bin.list && !only && row.last - row.first <= kBins * kChunkUnits) few = in_bin;
+    __syncthreads();  // the count is read
   }
   // Then by the order keys of the bin's logits, from the first bit in which they differ.
   uint32_t lo = 0xFFFFFFFFu, hi = 0;
-  row.each(few, [&](const auto& f, auto) {
+  row.each(in_bin, [&](const auto& f, auto) {
 #pragma unroll
     for (uint32_t i = 0; i < sizeof(f) / sizeof(float); ++i) {
       const bool in = f[i] > floor && coarse(f[i]) == bin;
@@ -780,7 +791,7 @@ __device__ __forceinline__ void find_edge(SampleShared& s, ExactShared& m, const
     const int step = min(left, 8);
     const int shift = left - step;
     // The largest digit first: digits are counted from the top.
-    find_bin(s, m.bins, row, few, weigh, [&](unsigned long long) { return goal; }, [&](float v) {
+    find_bin(s, m.bins, row, in_bin, weigh, [&](unsigned long long) { return goal; }, [&](float v) {
       const uint32_t k = order_key(v);
       const bool in = v > floor && coarse(v) == bin && (left == 32 || (k >> left) == prefix);
       return in ? (int)((1u << step) - 1u - ((k >> shift) & ((1u << step) - 1u))) : -1;
@@ -836,6 +847,7 @@ __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const Sa
   uint32_t* chunk_ties = few.list ? m.bins.count : reinterpret_cast<ChunkSums*>(memory)->ties;
   unsigned long long mass = 0;
   uint32_t tied = 0;
+  const bool plain = !p.first() && !(p.min_p > 0.f);  // kept() is fixed_of()
   __syncthreads();
   if (few.list) {
     for (uint32_t c = threadIdx.x; c < chunk1 - chunk0; c += kRowThreads) {
@@ -872,10 +884,16 @@ __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const Sa
         float f[kUnit<T>];
         unpack<T>(raw[j], f);
 #pragma unroll
-        for (uint32_t i = 0; i < kUnit<T>; ++i) {
-          const unsigned long long one_w = row.kept(f[i], p);
-          w += f[i] > kept.edge ? one_w : 0;
-          e += edged && f[i] == kept.edge;
+        for (uint32_t i = 0; i < kUnit<T>; ++i) e += edged && f[i] == kept.edge;
+        if (plain) {
+          unsigned long long one_w[kUnit<T>];
+#pragma unroll
+          for (uint32_t i = 0; i < kUnit<T>; ++i) one_w[i] = row.fixed_of(f[i]);
+#pragma unroll
+          for (uint32_t i = 0; i < kUnit<T>; ++i) w += f[i] > kept.edge ? one_w[i] : 0;
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < kUnit<T>; ++i) w += f[i] > kept.edge ? row.kept(f[i], p) : 0;
         }
       }
 #pragma unroll
@@ -981,7 +999,7 @@ __device__ __forceinline__ bool token_of_largest(SampleShared& s, const SampleRo
     keep = heavy;
   }
   if (!whole) return false;
-  const unsigned long long w = i < keep ? (p.first() && fixed == 0 && y > -1075.0 ? 1 : fixed) : 0;
+  const unsigned long long w = i < keep ? (p.first() && fixed == 0 && y > kNoWeight ? 1 : fixed) : 0;
   const unsigned long long sum = block_sum(w, s.scan);
   const unsigned long long need = p.need(sum);
   s.weight[i] = w;
@@ -1012,7 +1030,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   uint32_t chunk0, chunk1;
   split_units(chunks, cluster.rank, cluster.blocks, chunk0, chunk1);
   SampleRow<T> row{walk, chunk0 * kChunkUnits, min(chunk1 * kChunkUnits, walk.units), 0.f, 1.0 / (double)p.t,
-                   1.442695040888963407360 / (double)p.t, s.roots};
+                   16.0 * 1.442695040888963407360 / (double)p.t, 0.0, s.roots};
   row.first = min(row.first, row.last);
   float2* soft = reinterpret_cast<float2*>(memory + kTopDepth * kStepBytes);
   TopTold* told = reinterpret_cast<TopTold*>(soft + ((chunks + 1) & ~1u));
@@ -1086,6 +1104,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   for (uint32_t i = c0; i < c1; ++i) m = fmaxf(m, soft[i].x);
   m = block_max(m, reinterpret_cast<float*>(s.sums));
   row.m = m;
+  row.log2_m = -(double)m * row.log2_t;
   // 2^((x - m) c) of a chunk in 64 bits, with the c that its sum has.
   auto chunk_sum = [&](uint32_t i) {
     const float2 t = soft[i];
@@ -1207,7 +1226,11 @@ extern "C" int ws_sample(const ws_rows* logits, const float* uniform, const ws_s
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const uint32_t blocks = blocks_a_row(x);
+        // Where no token is dropped, some rows have all their tokens weighed as integers, 50 us for one block: more blocks for each
+        // (256 x 151936 fp32: 119 us with one, 79 with four).
+        const bool all_kept = !sampling->temperature_each && !sampling->top_k_each && !sampling->top_p_each && !sampling->min_p_each &&
+                              sampling->temperature > 0.f && sampling->top_k <= 0 && sampling->top_p >= 1.f && !(sampling->min_p > 0.f);
+        const uint32_t blocks = blocks_a_row(x, 0, all_kept ? 4 * kFewBlocks : kFewBlocks);
         const uint32_t chunks = (x.set.vocab + 2 * kUnit<T> - 2) / kChunk<T> + 1;  // at most, with the row's head
         return launch_rows<sample_kernel<T>>(x.rows, blocks, kTopDepth * kStepBytes + ((chunks + 1) & ~1u) * sizeof(float2) + (blocks > 1 ? sizeof(TopTold) : 0),
                                              device, stream, x.set, uniform, *sampling, tokens, logprobs);

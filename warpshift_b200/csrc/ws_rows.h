@@ -587,13 +587,16 @@ cudaError_t by_type(int dtype, F&& f) {
 }
 
 // How many blocks (a cluster: 1, 2, 4 or 8) share each row. Every block costs some microseconds beside its share of the row, so that
-// many rows go to one block each; kernels that write as much as they read gain from smaller shares, down to `share` KiB (0: one block).
-// Fewer rows than two blocks for each of 148 SMs are split until there are that many blocks, down to 16 KiB a block.
-inline uint32_t blocks_a_row(const RowArgs& x, uint32_t share = 0) {
+// many rows go to one block each (loss forward of 2048 x 128256 bf16: 84 us, 96 with two blocks a row); kernels that write as much as
+// they read gain from smaller shares, down to `share` KiB (backward of these: 175 us with one block, 164 with four). Rows are split further
+// until there are `most` blocks, down to 16 KiB a block: two for each of 148 SMs (top 64 of 64 x 128256: 14 us with four blocks a row, 18 with
+// one, 21 with eight).
+constexpr uint32_t kFewBlocks = 296;
+inline uint32_t blocks_a_row(const RowArgs& x, uint32_t share = 0, uint32_t most = kFewBlocks) {
   const uint32_t kib = x.set.vocab / 1024 * (x.dtype == WS_DTYPE_FP32 ? 4u : 2u);
   uint32_t c = 1;
   while (c < 8 && share && kib >= 2 * c * share) c *= 2;
-  while (c < 8 && (uint64_t)x.rows * c * 2 <= 296 && kib >= 2 * c * 16) c *= 2;
+  while (c < 8 && (uint64_t)x.rows * c * 2 <= most && kib >= 2 * c * 16) c *= 2;
   return c;
 }
 
