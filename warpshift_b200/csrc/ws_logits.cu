@@ -739,7 +739,7 @@ __device__ __forceinline__ void find_edge(SampleShared& s, ExactShared& m, const
       uint32_t mask = 0;
 #pragma unroll
       for (uint32_t i = 0; i < n; ++i) mask |= (f[i] > floor && (only ? coarse(f[i]) == bin : coarse(f[i]) <= bin) ? 1u : 0u) << i;
-      if (!mask) return;
+      if (!mask || s.top.count > kCandidates) return;  // too many already
       uint32_t i0 = atomicAdd(&s.top.count, (uint32_t)__popc(mask));
 #pragma unroll
       for (uint32_t i = 0; i < n; ++i) {
@@ -810,7 +810,7 @@ __device__ __forceinline__ void find_edge(SampleShared& s, ExactShared& m, const
 // The row's token from integer weights of all its tokens, by the whole cluster: into s.token of the block that holds it.
 // `memory`: what the ring left, for the counts. `few`: the block's part of the first top-k, if they are known.
 template <class T>
-__device__ __noinline__ void exact_token(SampleShared& s, void* memory, const SampleRow<T>& row, const SampleSettings& p, Few few, uint32_t vocab) {
+__device__ __noinline__ void exact_token(SampleShared& s, void* memory, const SampleRow<T> row, const SampleSettings p, Few few, uint32_t vocab) {
   cg::cluster_group cluster = cg::this_cluster();
   ExactShared& m = *reinterpret_cast<ExactShared*>(memory);
   Kept kept;
@@ -1230,7 +1230,10 @@ extern "C" int ws_sample(const ws_rows* logits, const float* uniform, const ws_s
         // (256 x 151936 fp32: 119 us with one, 79 with four).
         const bool all_kept = !sampling->temperature_each && !sampling->top_k_each && !sampling->top_p_each && !sampling->min_p_each &&
                               sampling->temperature > 0.f && sampling->top_k <= 0 && sampling->top_p >= 1.f && !(sampling->min_p > 0.f);
-        const uint32_t blocks = blocks_a_row(x, 0, all_kept ? 4 * kFewBlocks : kFewBlocks);
+        // Settings of each row's own bring such rows, too, and others that need as much, and the call ends with the slowest (128 x 128256
+        // bf16, all kinds of settings: 311 us with one block, 145 with four).
+        const bool each_own = sampling->temperature_each || sampling->top_k_each || sampling->top_p_each || sampling->min_p_each;
+        const uint32_t blocks = blocks_a_row(x, each_own ? 56 : 0, all_kept ? 4 * kFewBlocks : kFewBlocks);
         const uint32_t chunks = (x.set.vocab + 2 * kUnit<T> - 2) / kChunk<T> + 1;  // at most, with the row's head
         return launch_rows<sample_kernel<T>>(x.rows, blocks, kTopDepth * kStepBytes + ((chunks + 1) & ~1u) * sizeof(float2) + (blocks > 1 ? sizeof(TopTold) : 0),
                                              device, stream, x.set, uniform, *sampling, tokens, logprobs);
