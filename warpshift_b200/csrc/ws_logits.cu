@@ -635,6 +635,15 @@ __device__ __forceinline__ void find_in_chunk(SampleShared& s, const SampleRow<T
   }
 }
 
+// *p += w in shared memory, by its halves: two additions of 32 bits, the second one often 0, take less than one of 64, which is a
+// loop of exchanges.
+__device__ __forceinline__ void add_shared(unsigned long long* p, unsigned long long w) {
+  uint32_t* half = reinterpret_cast<uint32_t*>(p);
+  const uint32_t low = (uint32_t)w, old = atomicAdd(half, low);
+  const uint32_t high = (uint32_t)(w >> 32) + (old + low < old ? 1u : 0u);
+  if (high) atomicAdd(half + 1, high);
+}
+
 // One counting pass: digit(logit) in [0, kBins) for those that take part, or -1; in every bin how many they are and, where
 // `weigh`, their weight. Finds the lowest digit at which the running total (of counts, or of weights where `weigh`) reaches
 // target(total of all): s.found_*. A target of 0 asks for none. Returns the total. The last bin, which may take most of a row, is
@@ -667,7 +676,7 @@ __device__ __forceinline__ unsigned long long find_bin(SampleShared& s, Bins& bi
       }
 #pragma unroll
       for (uint32_t i = 0; i < n; ++i)
-        if ((uint32_t)d[i] < kBins - 1 && w[i]) atomicAdd(&bins.mass[d[i]], w[i]);
+        if ((uint32_t)d[i] < kBins - 1 && w[i]) add_shared(&bins.mass[d[i]], w[i]);
     }
 #pragma unroll
     for (uint32_t i = 0; i < n; ++i)
@@ -860,7 +869,7 @@ __device__ __noinline__ void exact_token(SampleShared& s, void* memory, const Sa
       const uint32_t c = (0xFFFFFFFFu - (uint32_t)few.list[i] + row.walk.head) / kChunk<T> - chunk0;
       if (v > kept.edge) {
         const unsigned long long w = row.kept(v, p);
-        atomicAdd(&chunk_mass[c], w);
+        add_shared(&chunk_mass[c], w);
         mass += w;
       } else if (v == kept.edge) {
         atomicAdd(&chunk_ties[c], 1u);
