@@ -110,6 +110,94 @@ def test_masks_and_records_with_gaps(cuda_device, dtype, tail) -> None:
     check(x, ids, logprobs, tail=tail)
 
 
+@pytest.mark.parametrize("rows,vocab", [(3, 70001), (40, 70001), (100, 40001), (160, 20001)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("tail", ["drop", "renormalize"])
+def test_rows_split_over_blocks(cuda_device, dtype, rows, vocab, tail) -> None:
+    """Long rows of a small batch go to clusters of 2, 4 and 8 blocks; many rows to one block each."""
+    t = TYPES[dtype]
+    ids, logprobs = record(rows, vocab, 200, seed=rows)
+    x = peaked(rows, vocab, t, seed=vocab)
+    weights = torch.ones(rows, device="cuda")
+    weights[1] = 0
+    if rows > 9:
+        x[2] = -torch.inf
+        x[3] = torch.finfo(t).min
+        x[4, vocab // 3 :] = -torch.inf
+        ids[4] %= vocab // 3
+        x[5, ids[5, 0]] = -torch.inf
+        ids[6] = -1
+        ids[7] = 33333 % vocab
+        ids[8, 100:] = ids[8, :100]
+    check(x[:30], ids[:30], logprobs[:30], weights=weights[:30], tail=tail, temperature=0.8)
+    if rows > 30:
+        check(x, ids, logprobs, weights=weights, tail=tail, grad_out=torch.randn(rows, generator=torch.Generator().manual_seed(2)).to("cuda"))
+
+
+def test_the_longest_rows(cuda_device) -> None:
+    x = peaked(2, 1 << 20, torch.float32, seed=3)
+    ids, logprobs = record(2, 1 << 20, 100, seed=4)
+    check(x, ids, logprobs)
+    loss, grad = distill.top_logprob_loss_and_grad(x[0].expand(200, 1 << 20), ids[0].expand(200, 100), logprobs[0].expand(200, 100))
+    want, want_grad = distill.top_logprob_loss_and_grad(x[:1], ids[:1], logprobs[:1])
+    torch.testing.assert_close(loss, want.expand(200), rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(grad[[0, 77, 199]], want_grad.expand(3, 1 << 20), rtol=1e-4, atol=1e-9)
+
+
+def test_rows_beyond_32_bits(cuda_device) -> None:
+    buffer = torch.empty((1 << 32) + 40000, dtype=torch.bfloat16, device="cuda")
+    x = buffer.as_strided((3, 9001), ((1 << 31) + 9001, 1))
+    x.copy_(peaked(3, 9001, torch.bfloat16, seed=1))
+    ids, logprobs = record(3, 9001, 20, seed=5)
+    check(x, ids, logprobs)
+
+
+def test_saved_tensors_may_be_kept_elsewhere(cuda_device) -> None:
+    """Hooks on saved tensors (offloading to the host) give the backward pass other tensors than the forward pass had."""
+    x = peaked(5, 3001, torch.bfloat16, seed=1).requires_grad_(True)
+    ids, logprobs = record(5, 3001, 20, seed=2)
+    with torch.autograd.graph.save_on_cpu():
+        loss = distill.top_logprob_loss(x, ids, logprobs, weights=torch.full((5,), 0.5, device="cuda"))
+    filler = torch.full((1 << 20,), 7.0, device="cuda")
+    (grad,) = torch.autograd.grad(loss.sum(), x)
+    del filler
+    _, want = distill.top_logprob_loss_and_grad(x.detach(), ids, logprobs, weights=torch.full((5,), 0.5, device="cuda"))
+    torch.testing.assert_close(grad, want, rtol=2.0**-7, atol=1e-8)
+
+
+def test_backward_twice_and_changed_logits(cuda_device) -> None:
+    x = peaked(4, 999, torch.float32, seed=1).requires_grad_(True)
+    ids, logprobs = record(4, 999, 9, seed=2)
+    loss = distill.top_logprob_loss(x, ids, logprobs)
+    (first,) = torch.autograd.grad(loss.sum(), x, retain_graph=True)
+    (second,) = torch.autograd.grad(loss.sum(), x, retain_graph=True)
+    assert torch.equal(first, second)
+    (grad,) = torch.autograd.grad(loss.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        grad.sum().backward()
+    loss = distill.top_logprob_loss(x, ids, logprobs)
+    with torch.no_grad():
+        x.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+
+
+def test_two_steps_on_two_streams(cuda_device) -> None:
+    xs = [peaked(64, 20011, torch.bfloat16, seed=s) for s in (1, 2)]
+    ids, logprobs = record(64, 20011, 30, seed=3)
+    want = [distill.top_logprob_loss_and_grad(x, ids, logprobs) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(distill.top_logprob_loss_and_grad(xs[i], ids, logprobs))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for loss, grad in got[i]:
+            assert torch.equal(loss, want[i][0]) and torch.equal(grad, want[i][1])
+
+
 def test_rows_of_weight_zero_are_not_read(cuda_device) -> None:
     x = peaked(4, 999, torch.bfloat16, seed=1)
     ids, logprobs = record(4, 999, 5, seed=2)

@@ -90,6 +90,50 @@ def test_rows_of_any_stride_and_alignment(cuda_device, dtype) -> None:
     assert empty.ids.shape == (0, 4)
 
 
+# Long rows of a small batch go to clusters of 2, 4 and 8 blocks; many rows to one block each.
+SPLITS = [(3, 70001), (40, 70001), (100, 40001), (160, 20001)]
+
+
+@pytest.mark.parametrize("rows,vocab", SPLITS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_top_logprobs_of_split_rows(cuda_device, dtype, rows, vocab) -> None:
+    t = TYPES[dtype]
+    x = peaked(rows, vocab, t, seed=rows)
+    x[0] = -torch.inf
+    x[1, 5:] = -torch.inf
+    x[1, -3:] = 2.0
+    x[2] = torch.finfo(t).min
+    if rows > 9:
+        at = torch.arange(vocab, device="cuda")
+        x[3] = (at / 2000).to(t)
+        x[4] = (-at / 2000).to(t)
+        x[5] = 1.25
+        x[6, vocab // 2 :] = -torch.inf
+        x[7, 30000 % vocab] = torch.nan
+        x[8, 30000 % vocab] = torch.inf
+    check_top(x, 256)
+    check_top(x[:9], 20, temperature=0.5)
+    check_top(x[:9, 1:], 1)
+
+
+def test_top_logprobs_of_the_longest_rows(cuda_device) -> None:
+    x = peaked(2, 1 << 20, torch.float32, seed=3)
+    check_top(x, 100)
+    one_block = ops.top_logprobs(x[0].expand(200, 1 << 20), 100)
+    assert torch.equal(one_block.ids, ops.top_logprobs(x[:1], 100).ids.expand(200, 100))
+    with pytest.raises(ValueError):
+        ops.top_logprobs(torch.zeros(1, device="cuda").expand((1 << 20) + 1), 1)
+
+
+def test_rows_beyond_32_bits(cuda_device) -> None:
+    """Rows whose offset passes 2^32 elements, and 2^32 bytes."""
+    buffer = torch.empty((1 << 32) + 40000, dtype=torch.bfloat16, device="cuda")
+    x = buffer.as_strided((3, 9001), ((1 << 31) + 9001, 1))
+    x.copy_(peaked(3, 9001, torch.bfloat16, seed=1))
+    check_top(x, 30)
+    check_sample(x, torch.tensor([0.1, 0.5, 0.9], device="cuda"), top_p=0.9)
+
+
 def settings(rows: int, seed: int) -> dict[str, torch.Tensor]:
     g = torch.Generator().manual_seed(seed)
 
@@ -167,6 +211,42 @@ def test_sample_with_masked_logits(cuda_device, dtype, params) -> None:
     x[8, ::2] = -torch.inf
     for u in (0.0, 0.3, 0.7, 1 - 2.0**-24):
         check_sample(x, torch.full((9,), u, device="cuda"), **params)
+
+
+@pytest.mark.parametrize("rows,vocab", SPLITS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_sample_of_split_rows(cuda_device, dtype, rows, vocab) -> None:
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(rows)
+    x = peaked(rows, vocab, t, seed=vocab, scale=2.0)
+    if rows > 9:
+        at = torch.arange(vocab, device="cuda")
+        x[0] = -torch.inf
+        x[1, 5:] = -torch.inf
+        x[2] = torch.finfo(t).min
+        x[3] = (at / 2000).to(t)
+        x[4] = 1.25
+        x[5, : vocab // 2] = -torch.inf
+        x[6, 30000 % vocab] = torch.nan
+        x[7, 30000 % vocab] = torch.inf
+        x[8] = (at % 5 == 0).to(t)
+        x[9] = torch.randn(vocab, generator=g).to(t)
+        x[10] = torch.randn(vocab, generator=g).to(t) * 0.01
+    uniform = torch.rand(rows, generator=g).to("cuda")
+    uniform[0::7] = 0.0
+    check_sample(x[:60], uniform[:60], **{n: p[:60] for n, p in settings(rows, vocab).items()})
+    for params in ({}, {"top_p": 0.8}, {"top_k": 500, "top_p": 0.9}, {"top_k": 5000}, {"min_p": 0.2, "temperature": 1.5}, {"temperature": 0.0}):
+        check_sample(x[:11], uniform[:11], **params)
+
+
+def test_sample_of_the_longest_rows(cuda_device) -> None:
+    x = peaked(1, 1 << 20, torch.float32, seed=3)
+    u = torch.rand(200, generator=torch.Generator().manual_seed(1)).to("cuda")
+    for params in ({}, {"top_p": 0.95}, {"top_k": 5000}):
+        check_sample(x, u[:1], **params)
+        many = ops.sample(x.expand(200, 1 << 20), u, **params).tokens  # a block for each row
+        one = torch.cat([ops.sample(x, u[i : i + 1], **params).tokens for i in range(200)])  # eight for each
+        assert torch.equal(many, one)
 
 
 def test_sample_uniform_out_of_range_takes_the_ends(cuda_device) -> None:

@@ -88,10 +88,21 @@ def _backward(ctx, grad_loss):
     index = logits.get_device()
     _lib.check(_lib.load().ws_distill_backward(byref(rows), byref(record), stats.data_ptr(), grad_loss.data_ptr(), outer, inner,
                                                byref(out), index, stream_of(index)))
+    if torch.is_grad_enabled():  # under create_graph
+        grad = _Once.apply(grad, logits)
     return grad, None, None, None, None, None
 
 
-_backward_once = torch.autograd.function.once_differentiable(_backward)
+class _Once(torch.autograd.Function):
+    """A gradient that is not to be differentiated again, with respect to the logits it is a function of."""
+
+    @staticmethod
+    def forward(ctx, grad, logits):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("top_logprob_loss can be differentiated once")
 
 
 class _TopLogprobLoss(torch.autograd.Function):
@@ -108,10 +119,7 @@ class _TopLogprobLoss(torch.autograd.Function):
         ctx.settings = temperature, tail
         return loss
 
-    @staticmethod
-    def backward(ctx, grad_loss):
-        # Under create_graph the result is marked as differentiable no further, which costs 10 us that other calls need not pay.
-        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_loss)
+    backward = staticmethod(_backward)
 
 
 def top_logprob_loss(
