@@ -222,43 +222,74 @@ class DenseGrad {
     folded_ = sizeof(T) == 2 && a_ > 1e-30f && a_ < 1e30f && fabsf(r_) < 100.f;
     if (folded_) r_ -= log2f(scale_);
   }
-  // One step's units, which begin at unit u0; inside: they are wholly the row's.
-  __device__ __forceinline__ void write(const Batch<T>& b, uint32_t u0, bool inside) const {
-    uint4* out = reinterpret_cast<uint4*>(out_) + Batch<T>::unit(u0, 0);
-    const uint64_t cc = pair(c_, c_), nr = pair(-r_, -r_), aa = pair(scale_, scale_);
+  // All steps from unit `first`: read(batch, u0) gives the step's logits, inside(u0) tells whether its units are wholly the row's.
+  template <class R, class I>
+  __device__ __forceinline__ void write(uint32_t first, R&& read, I&& inside) const {
+    if (wide_ && one_step_) {
+      if (folded_) write_wide<true>(first, read, inside);
+      else write_wide<false>(first, read, inside);
+      return;
+    }
+    for (uint32_t u0 = first; u0 < last_; u0 += Batch<T>::kSpan) {
+      Batch<T> b;
+      read(b, u0);
+#pragma unroll 1
+      for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+        const uint32_t u = Batch<T>::unit(u0, j);
+        if (u >= last_) continue;
+        uint4 raw = b.raw[0];
 #pragma unroll
-    for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
-      float f[kUnit<T>];
-      unpack<T>(b.raw[j], f);
-      if (one_step_) {
+        for (uint32_t q = 1; q < Batch<T>::kUnits; ++q) raw = q == j ? b.raw[q] : raw;
+        float f[kUnit<T>];
+        unpack<T>(raw, f);
 #pragma unroll
-        for (uint32_t i = 0; i < kUnit<T>; i += 2) {
-          const float2 e = unpair(fma2(pair(f[i], f[i + 1]), cc, nr));
-          f[i] = ex2(e.x);
-          f[i + 1] = ex2(e.y);
-        }
-        if (!folded_) {
-#pragma unroll
-          for (uint32_t i = 0; i < kUnit<T>; i += 2) {
-            const float2 e = unpair(mul2(pair(f[i], f[i + 1]), aa));
-            f[i] = e.x;
-            f[i + 1] = e.y;
-          }
-        }
-      } else {
-#pragma unroll
-        for (uint32_t i = 0; i < kUnit<T>; ++i) f[i] = a_ * ex2((f[i] - m_) * c_);
+        for (uint32_t i = 0; i < kUnit<T>; ++i) f[i] = one_step_ ? scale_ * ex2(fmaf(f[i], c_, -m_ * c_)) : a_ * ex2((f[i] - m_) * c_);
+        write_edge(walk_, out_, u, pack<T>(f));
       }
-      const uint4 v = pack<T>(f);
-      const uint32_t u = Batch<T>::unit(u0, j);
-      if (wide_ && (inside || (u < last_ && walk_.whole(u))))
-        out[j * 32] = v;
-      else if (u < last_)
-        write_edge(walk_, out_, u, v);
     }
   }
 
  private:
+  template <bool kFolded, class R, class I>
+  __device__ __forceinline__ void write_wide(uint32_t first, R&& read, I&& inside) const {
+    const uint64_t cc = pair(c_, c_), nr = pair(-r_, -r_), aa = pair(scale_, scale_);
+    uint4* out = reinterpret_cast<uint4*>(out_) + Batch<T>::unit(first, 0);
+    for (uint32_t u0 = first; u0 < last_; u0 += Batch<T>::kSpan, out += Batch<T>::kSpan) {
+      Batch<T> b;
+      read(b, u0);
+#pragma unroll
+      for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+        float f[kUnit<T>];
+        unpack<T>(b.raw[j], f);
+#pragma unroll
+        for (uint32_t i = 0; i < kUnit<T>; i += 2) {
+          float2 e = unpair(fma2(pair(f[i], f[i + 1]), cc, nr));
+          e.x = ex2(e.x);
+          e.y = ex2(e.y);
+          if (!kFolded) e = unpair(mul2(pair(e.x, e.y), aa));
+          f[i] = e.x;
+          f[i + 1] = e.y;
+        }
+        b.raw[j] = pack<T>(f);
+      }
+      if (inside(u0)) {
+#pragma unroll
+        for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) out[j * 32] = b.raw[j];
+      } else {
+#pragma unroll 1
+        for (uint32_t j = 0; j < Batch<T>::kUnits; ++j) {
+          const uint32_t u = Batch<T>::unit(u0, j);
+          uint4 raw = b.raw[0];
+#pragma unroll
+          for (uint32_t q = 1; q < Batch<T>::kUnits; ++q) raw = q == j ? b.raw[q] : raw;
+          if (u >= last_) continue;
+          if (walk_.whole(u)) out[j * 32] = raw;
+          else write_edge(walk_, out_, u, raw);
+        }
+      }
+    }
+  }
+
   const RowWalk<T>& walk_;
   T* out_;
   uint32_t last_;
@@ -362,13 +393,16 @@ __global__ void __launch_bounds__(kRowThreads, 4)
   }
   RowGrad g{st.x, factor * st.y, factor, 0.f};
   const DenseGrad<T> dense(walk, out, last, g, r.c);
-  for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
-    Batch<T> b;
+  bool looked_up = false;
+  dense.write(first, [&](Batch<T>& b, uint32_t u0) {
+    if (u0 != first) {
+      ring.advance();
+      if (!looked_up) e.look_up(src, x.vocab);
+      looked_up = true;
+    }
     ring.read(b);
-    dense.write(b, u0, ring.inside(u0));
-    ring.advance();
-    if (u0 == first) e.look_up(src, x.vocab);
-  }
+  }, [&](uint32_t u0) { return ring.inside(u0); });
+  if (!looked_up) e.look_up(src, x.vocab);
   put_record(r, e, record, r.renormalize);
   __syncthreads();
   const float share = record_share(r, e, record, walk, first, last);
@@ -425,19 +459,13 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   } else if (last - first <= kStepDepth * Batch<T>::kSpan) {
     // The second pass from shared memory, where the block's share still is.
     uint32_t slot = 0;
-    for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan, ++slot) {
-      Batch<T> b;
-      ring.again(slot, b);
-      dense.write(b, u0, ring.inside(u0));
-    }
+    dense.write(first, [&](Batch<T>& b, uint32_t) { ring.again(slot++, b); }, [&](uint32_t u0) { return ring.inside(u0); });
   } else {
     Ring<T, kStepDepth> second(ring_memory, walk, first, last);
-    for (uint32_t u0 = first; u0 < last; u0 += Batch<T>::kSpan) {
-      Batch<T> b;
+    dense.write(first, [&](Batch<T>& b, uint32_t u0) {
+      if (u0 != first) second.advance();
       second.read(b);
-      dense.write(b, u0, ring.inside(u0));
-      second.advance();
-    }
+    }, [&](uint32_t u0) { return second.inside(u0); });
   }
   if (g.dense != 0.f) write_record(r, e, share, walk, out, g);
   if (cluster.rank == 0 && threadIdx.x == 0) loss[row] = w * row_loss(r, t, soft);
