@@ -46,8 +46,6 @@ int check_rows(const ws_rows* rows, const char* what, RowArgs* out) {
 
 namespace {
 
-namespace cg = cooperative_groups;
-
 struct Record {
   const void* ids;
   const float* logprobs;
