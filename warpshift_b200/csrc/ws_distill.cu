@@ -11,6 +11,11 @@
 // tokens of the record are a correction: the dense part of a row is written first and
 // the elements named by the record again behind a block barrier, each once, by the
 // first entry that names it.
+//
+// All three kernels are bound by HBM where rows are many. 4096 x 151936 bf16, k = 32: forward
+// 187 us (6.7 TB/s), backward 370 us (6.7 TB/s, read and write). The one-launch kernel
+// waits between its passes for the row's sum: 2048 x 128256 bf16 216 us, where reading and writing once
+// take 160; its second pass comes from L2, or from shared memory where a block's share is 64 KiB at most.
 #include <algorithm>
 #include <string>
 
@@ -56,7 +61,8 @@ struct Record {
   float inv_t;  // 1 / temperature
 };
 
-constexpr uint32_t kDepth = 3;      // steps in flight of the kernels that read a row once
+// Steps in flight of the kernels that read a row once (2048 x 128256 bf16, forward: 90, 85 and 90 us with 2, 3 and 4).
+constexpr uint32_t kDepth = 3;
 constexpr uint32_t kStepDepth = 4;  // of the one that reads it twice: a block's share up to 64 KiB stays
 
 // Entry `threadIdx.x` of a row's record and the logit of its token; a token id of -1 has no mass. Loaded in two parts, the second of
