@@ -65,6 +65,10 @@ struct Record {
 constexpr uint32_t kDepth = 3;
 constexpr uint32_t kStepDepth = 4;  // of the one that reads it twice: a block's share up to 64 KiB stays
 
+// Every block of a row goes over the whole record: with long ones a row has fewer blocks (333 x 50001 fp32, k = 256, one and two blocks:
+// backward 42 and 48 us, both in one launch 55 and 64).
+constexpr uint32_t kShortRecord = 64;
+
 // Entry `threadIdx.x` of a row's record and the logit of its token; a token id of -1 has no mass. Loaded in two parts, the second of
 // which needs the first, so that a kernel can read its row in between.
 struct Entry {
@@ -545,7 +549,7 @@ extern "C" int ws_distill_backward(const ws_rows* logits, const ws_teacher* teac
     if (x.rows == 0) return (int)WS_OK;
     if (!stats || !grad_loss) return fail(WS_ERR_INVALID, "null pointer");
     if ((uintptr_t)stats % 8) return fail(WS_ERR_INVALID, "stats must be 8-byte aligned");
-    const uint32_t pieces = blocks_a_row(x, 56);
+    const uint32_t pieces = blocks_a_row(x, r.k <= kShortRecord ? 56 : 112);
     DeviceGuard guard(device);
     cudaError_t e = guard.error();
     if (e == cudaSuccess)
@@ -574,7 +578,7 @@ extern "C" int ws_distill_step(const ws_rows* logits, const ws_teacher* teacher,
     if (e == cudaSuccess)
       e = by_type(x.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows<distill_step_kernel<T>>(x.rows, blocks_a_row(x, 96), kStepDepth * kStepBytes, device, stream, x.set, r, loss, dx.set);
+        return launch_rows<distill_step_kernel<T>>(x.rows, blocks_a_row(x, r.k <= kShortRecord ? 96 : 192), kStepDepth * kStepBytes, device, stream, x.set, r, loss, dx.set);
       });
     return done(e, "distill step");
   });
