@@ -455,6 +455,7 @@ constexpr uint32_t kChunk = kChunkUnits * kUnit<T>;
 constexpr uint32_t kChunks = WS_MAX_VOCAB / kChunk<float> + 1;
 constexpr double kWeightOne = 4398046511104.0;  // 2^42
 constexpr double kSumError = 1.0 / 131072;
+constexpr uint32_t kNucleus = 200;  // tokens at hand where top-k does not say: of 256, some 290 candidates would have to be sorted in 512 places
 constexpr double kNoWeight = -16.0 * 1075.0;  // 16 log2 of what 64 bits round to 0
 
 struct Bins {
@@ -652,7 +653,7 @@ __device__ __forceinline__ void add_shared(unsigned long long* p, unsigned long 
   if (high) atomicAdd(half + 1, high);
 }
 
-// One counting pass: digit(logit) in [0, kBins) for those that take part, or -1; in every bin how many they are and, where
+// One counting pass: digit(logit) in [0, kBins) for those that take part, or -1; in every bin how many they are or, where
 // `weigh`, their weight. Finds the lowest digit at which the running total (of counts, or of weights where `weigh`) reaches
 // target(total of all): s.found_*. A target of 0 asks for none. Returns the total. The last bin, which may take most of a row, is
 // counted in registers.
@@ -685,10 +686,11 @@ __device__ __forceinline__ unsigned long long find_bin(SampleShared& s, Bins& bi
 #pragma unroll
       for (uint32_t i = 0; i < n; ++i)
         if ((uint32_t)d[i] < kBins - 1 && w[i]) add_shared(&bins.mass[d[i]], w[i]);
-    }
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < n; ++i)
-      if ((uint32_t)d[i] < kBins - 1) atomicAdd(&bins.count[d[i]], 1u);
+      for (uint32_t i = 0; i < n; ++i)
+        if ((uint32_t)d[i] < kBins - 1) atomicAdd(&bins.count[d[i]], 1u);
+    }
   });
   tail_count = (uint32_t)block_sum((unsigned long long)tail_count, s.scan);
   tail_mass = block_sum(tail_mass, s.scan);
@@ -720,7 +722,6 @@ __device__ __forceinline__ unsigned long long find_bin(SampleShared& s, Bins& bi
     if (before < goal && before + in >= goal) {
       s.found_bin = threadIdx.x * kMine + j;
       s.found_before = before;
-      s.found_count = count[j];
     }
     before += in;
   }
@@ -743,7 +744,6 @@ __device__ __forceinline__ void find_edge(SampleShared& s, ExactShared& m, const
   if (goal == 0) return;  // the same for the whole cluster
   const int bin = (int)s.found_bin;
   goal -= s.found_before;
-  uint32_t at = s.found_count;
   // Nothing below this bin is kept: if what is above is few in this block, the passes to come need not go over the row; if only the bin's own
   // tokens are, those of this function need not. The edge lies above the floor, so that tokens at the floor itself are not kept. The list has
   // the counts of up to kBins chunks beside it.
@@ -814,14 +814,14 @@ __device__ __forceinline__ void find_edge(SampleShared& s, ExactShared& m, const
       return in ? (int)((1u << step) - 1u - ((k >> shift) & ((1u << step) - 1u))) : -1;
     });
     goal -= s.found_before;
-    at = s.found_count;
     prefix = (left == 32 ? 0u : prefix << step) | ((1u << step) - 1u - s.found_bin);
     left = shift;
     __syncthreads();  // found_* is read
   }
   kept.edge = key_value(prefix);
+  // What is left of the target lies within the weight of the tokens at the edge, which all weigh the same.
   const unsigned long long one = row.fixed_of(kept.edge);
-  kept.ties = weigh ? (uint32_t)min((unsigned long long)at, (goal + one - 1) / max(one, 1ull)) : (uint32_t)goal;
+  kept.ties = (uint32_t)(weigh ? (goal + one - 1) / max(one, 1ull) : goal);
 }
 
 // The row's token from integer weights of all its tokens, by the whole cluster: into s.token of the block that holds it.
@@ -1053,10 +1053,10 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   TopTold* told = reinterpret_cast<TopTold*>(soft + ((chunks + 1) & ~1u));
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const bool dropping = (p.top_k >= 1 && p.top_k < (int64_t)x.vocab) || p.top_p < 1.f || p.min_p > 0.f;
-  // The largest logits, in order: as many as top-k asks for, or WS_TOP_MAX_K. A larger top-k is left to exact_token, which up to
+  // The largest logits, in order: as many as top-k asks for, or kNucleus. A larger top-k is left to exact_token, which up to
   // kMostCollected gets a list.
   const bool many = p.top_k > WS_TOP_MAX_K && p.top_k <= kMostCollected && p.top_k < (int64_t)x.vocab;
-  const uint32_t k = p.top_k >= 1 && p.top_k <= kMostCollected ? (uint32_t)p.top_k : WS_TOP_MAX_K;
+  const uint32_t k = p.top_k >= 1 && p.top_k <= kMostCollected ? (uint32_t)p.top_k : kNucleus;
   Few few;
 
   Ring<T, kTopDepth> ring(memory, walk, row.first, row.last);
