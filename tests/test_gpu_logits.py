@@ -330,3 +330,18 @@ def test_answer_records_of_a_model_switched_there_and_back(cuda_device) -> None:
     delta.apply(reverse=False)
     assert verify.compare_answers(native, other) == [] and verify.compare_answers(before, answers()) == []
     assert verify.compare_answers(before, other)
+
+
+@pytest.mark.parametrize("temperature", [1e-38, 1e-30, 1e-6, 1e6, 1e30, float("inf")])
+def test_sample_at_the_ends_of_temperature(cuda_device, temperature) -> None:
+    g = torch.Generator().manual_seed(8)
+    x = peaked(4, 3001, torch.float32, seed=8)
+    x[1] = torch.finfo(torch.float32).max * (torch.rand(3001, generator=g) * 2 - 1).to("cuda")
+    x[2] = torch.arange(3001, device="cuda") * 2.0**-20 + 1e4
+    x[3] = torch.where(torch.arange(3001) % 7 == 0, 1e-40, 0.0).to("cuda")
+    for u in (0.0, 0.2, 0.9):
+        for params in ({}, {"top_p": 0.7}, {"top_k": 900}, {"min_p": 0.5}):
+            check_sample(x[:3], torch.full((3,), u, device="cuda"), temperature=temperature, **params)
+    # Logits below the smallest normal number still order the tokens.
+    assert int(ops.sample(x[3:], torch.full((1,), 0.5, device="cuda"), temperature=0.0).tokens) == 0
+    assert ops.top_logprobs(x[3:], 3).ids.tolist() == [[0, 7, 14]]
