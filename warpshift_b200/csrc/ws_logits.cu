@@ -1041,7 +1041,8 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   cluster.started();
   const uint32_t r = cluster.row();
   const SampleSettings p(sampling, uniform, r);
-  const float c = fminf(kLog2e / p.t, 3e38f);
+  // Finite and above 0, so that a logit of -inf has no weight at an infinite temperature, either.
+  const float c = fmaxf(fminf(kLog2e / p.t, 3e38f), 1.4e-45f);
   const RowWalk<T> walk(row_ptr<T>(x, r), x.vocab);
   const uint32_t chunks = (walk.units + kChunkUnits - 1) / kChunkUnits;
   uint32_t chunk0, chunk1;
